@@ -204,6 +204,96 @@ NDL_API int ndl_attention_paged_noalloc(const int8_t *q, const float *qs, const 
                                         int slots, int max_pages, const uint8_t *pool, size_t page_bytes,
                                         int num_pages, int layer, float *out, int *status, void *stream);
 
+/* ---- Rows, attention and logits over caller-owned pages ------------------
+ * Operators of the serving path for hosts that own their device buffers:
+ * write a request's keys and values into the pages of ndl_attention_paged's
+ * layout, attend to them with a whole prompt or with single tokens, and
+ * adjust the logits before they are sampled.  No counterpart in the
+ * reference, whose prompts run as decode rows.
+ *
+ * Element types of q, k, v and out; 64 dims a head, the rows' heads and dims
+ * contiguous, `*_stride` elements between rows (a multiple of 16 bytes, so a
+ * fused projection's columns can be passed as they lie; rows 16-byte
+ * aligned).  The cache arguments are those of ndl_attention_paged with
+ * kv_heads records a layer, except that a slot may have any number of pages.
+ * status (nullable, device int) receives 2 for an out-of-range slot,
+ * position, length or page (the row's outputs are then NaN, other rows are
+ * unaffected) and 1 for a timed-out wait.  Device pointers, asynchronous on
+ * `stream`, which belongs to the current device; nothing is allocated. */
+enum { NDL_TYPE_F32 = 0, NDL_TYPE_F16 = 1, NDL_TYPE_BF16 = 2 };
+
+/* Rows of keys and values into the pages: row r of every kv head goes to
+ * position row_pos[r] of slot row_slot[r], quantized per (row, head) as
+ * ndl_quantize_rows does (the codes and scales the engine's own steps store
+ * for the same 64 values).  A negative position marks a padding row, which
+ * is not written.  The rows of one call go to distinct positions: where two
+ * name the same one its content is undefined.  A bad row writes nothing. */
+NDL_API int ndl_kv_append(const void *k, long long k_stride, const void *v, long long v_stride, int type,
+                          const int32_t *row_slot, const int32_t *row_pos, int rows, int kv_heads,
+                          const int32_t *page_table, int slots, int max_pages, uint8_t *pool, size_t page_bytes,
+                          int num_pages, int layer, int *status, void *stream);
+/* The rows back: code * scale in fp32, rounded to the type.  A padding row
+ * (negative position) gives zeros, a bad one NaN. */
+NDL_API int ndl_kv_gather(const int32_t *row_slot, const int32_t *row_pos, int rows, int kv_heads,
+                          const int32_t *page_table, int slots, int max_pages, const uint8_t *pool, size_t page_bytes,
+                          int num_pages, int layer, void *k, long long k_stride, void *v, long long v_stride, int type,
+                          int *status, void *stream);
+
+/* Whole-prompt attention, causal, over packed sequences.  Rows seq_rows[s]
+ * .. seq_rows[s+1] (ascending offsets, seq_rows[0] >= 0) of q [rows][heads]
+ * [64] are sequence s's queries at positions seq_pos[s], seq_pos[s] + 1, ...
+ * of slot seq_slot[s], whose pages already hold the keys and values up to the
+ * last of them (ndl_kv_append), a shared or earlier prefix included.  Query
+ * head h reads kv head h / (heads / kv_heads).  With window w > 0 a query at
+ * position p attends to (p - w, p], else to [0, p]:
+ *   out = sum_j softmax_j(scale * q . k_j) v_j
+ * Scores, softmax and sums are in fp32; 16-bit types round the
+ * probabilities to fp16 before the second product, fp32 splits queries and
+ * probabilities into two fp16 parts.  Rows of no sequence are left as they
+ * are; a sequence whose offsets descend or leave [0, rows] is skipped with
+ * status 2. */
+NDL_API int ndl_attention_prompt(const void *q, long long q_stride, int type, const int32_t *seq_rows,
+                                 const int32_t *seq_slot, const int32_t *seq_pos, int sequences, int rows, int heads,
+                                 int kv_heads, float scale, int window, const int32_t *page_table, int slots,
+                                 int max_pages, const uint8_t *pool, size_t page_bytes, int num_pages, int layer,
+                                 void *out, long long out_stride, int *status, void *stream);
+
+/* Attention of single tokens: row r attends to positions [0, row_len[r]) of
+ * slot row_slot[r] (the last `window` of them with window > 0), its cache
+ * split over several thread blocks and the parts joined.  A row of length 0
+ * gives zeros.  Arithmetic as ndl_attention_prompt.  workspace: device
+ * memory of ndl_attention_split_workspace bytes, 16-byte aligned; calls that
+ * overlap on the GPU need one each.  Its contents need no set-up and mean
+ * nothing between calls. */
+NDL_API size_t ndl_attention_split_workspace(int rows, int heads, int kv_heads, int max_pages);
+NDL_API int ndl_attention_split(const void *q, long long q_stride, int type, const int32_t *row_slot,
+                                const int32_t *row_len, int rows, int heads, int kv_heads, float scale, int window,
+                                const int32_t *page_table, int slots, int max_pages, const uint8_t *pool,
+                                size_t page_bytes, int num_pages, int layer, void *out, long long out_stride,
+                                void *workspace, size_t workspace_bytes, int *status, void *stream);
+
+/* Penalties, biases and masks on logits x [rows][vocab] (ldx floats between
+ * rows) into y (may be x with the same stride; must not overlap it
+ * otherwise), for the samplers (ndl_sample_argmax masks by itself).  In
+ * this order, each step one IEEE operation:
+ *   repetition[row]: an id among the row's tokens: x > 0 ? x / r : x * r
+ *   frequency[row], presence[row]: an id that occurs n > 0 times among the
+ *     row's output tokens (those behind its first prompt_lens[row]; null: all
+ *     are output): x - f * n, then x - p
+ *   bias: the row's last entry for the id is added
+ *   mask: ids whose bit is clear, and ids >= 32 * words, become -inf
+ * Row r's tokens are tokens[token_offsets[r] .. token_offsets[r+1]), its bias
+ * entries bias_ids / bias_values [bias_offsets[r] .. bias_offsets[r+1]); ids
+ * outside the vocabulary are ignored.  Its mask is masks' row mask_index[r]
+ * (negative: none), without mask_index row r; a row past mask_rows is NaN
+ * with status 2.  Every list and penalty is nullable. */
+NDL_API int ndl_logits_process(const float *x, long long ldx, float *y, long long ldy, int rows, int vocab,
+                               const int32_t *tokens, int n_tokens, const int32_t *token_offsets,
+                               const int32_t *prompt_lens, const float *repetition, const float *frequency,
+                               const float *presence, const int32_t *bias_ids, const float *bias_values, int n_bias,
+                               const int32_t *bias_offsets, const uint32_t *mask, int mask_rows, int words,
+                               const int32_t *mask_index, int *status, void *stream);
+
 /* ------------------------------------------------------------------ */
 /* KernelTable conformance exports                                     */
 /* ------------------------------------------------------------------ */

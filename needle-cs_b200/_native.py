@@ -41,6 +41,20 @@ SIGNATURES = {
                                     c_void_p]),
     "ndl_attention_paged_noalloc": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_int,
                                             c_int, c_void_p, c_size_t, c_int, c_int, c_void_p, c_void_p, c_void_p]),
+    "ndl_kv_append": (c_int, [c_void_p, c_ll, c_void_p, c_ll, c_int, c_void_p, c_void_p, c_int, c_int, c_void_p, c_int,
+                              c_int, c_void_p, c_size_t, c_int, c_int, c_void_p, c_void_p]),
+    "ndl_kv_gather": (c_int, [c_void_p, c_void_p, c_int, c_int, c_void_p, c_int, c_int, c_void_p, c_size_t, c_int,
+                              c_int, c_void_p, c_ll, c_void_p, c_ll, c_int, c_void_p, c_void_p]),
+    "ndl_attention_prompt": (c_int, [c_void_p, c_ll, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int,
+                                     c_float, c_int, c_void_p, c_int, c_int, c_void_p, c_size_t, c_int, c_int,
+                                     c_void_p, c_ll, c_void_p, c_void_p]),
+    "ndl_attention_split_workspace": (c_size_t, [c_int, c_int, c_int, c_int]),
+    "ndl_attention_split": (c_int, [c_void_p, c_ll, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_float, c_int,
+                                    c_void_p, c_int, c_int, c_void_p, c_size_t, c_int, c_int, c_void_p, c_ll,
+                                    c_void_p, c_size_t, c_void_p, c_void_p]),
+    "ndl_logits_process": (c_int, [c_void_p, c_ll, c_void_p, c_ll, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p,
+                                   c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int,
+                                   c_int, c_void_p, c_void_p, c_void_p]),
     "ndl_engine_create": (c_int, [c_void_p, c_void_p, ctypes.POINTER(c_void_p)]),
     "ndl_engine_create_model": (c_int, [c_void_p, c_void_p, ctypes.POINTER(c_void_p)]),
     "ndl_whistle_create": (c_int, [c_void_p, c_int, ctypes.POINTER(c_void_p)]),

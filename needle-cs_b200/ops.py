@@ -170,3 +170,187 @@ def attention_paged(q8, qs, row_slot, row_pos, page_table, pool, page_bytes, lay
          pool.numel() // page_bytes, layer, _dev(out, torch.float32, "out"), ws_ptr, ws_bytes,
          _dev(status, torch.int32, "status") if status is not None else None, _stream())
     return out
+
+
+# ------------------------------- rows, attention and logits over own pages --
+
+_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
+def _type(t, name):
+    if not isinstance(t, torch.Tensor) or t.dtype not in _TYPES:
+        raise TypeError(f"{name} must be a float32, float16 or bfloat16 tensor")
+    return _TYPES[t.dtype]
+
+
+def _heads(t, dtype, name, device, shape=None):
+    """Address and row stride of a [rows, heads, 64] operand whose rows may be strided (a projection's columns)."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise TypeError(f"{name} must be a CUDA tensor")
+    if t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, not on {device}")
+    if t.dim() != 3 or t.shape[2] != 64 or (shape is not None and tuple(t.shape) != tuple(shape)):
+        raise ValueError(f"{name} must be [rows, heads, 64]{'' if shape is None else f' = {list(shape)}'}, got {list(t.shape)}")
+    rows, heads, _ = t.shape
+    if rows and heads and (t.stride(2) != 1 or (heads > 1 and t.stride(1) != 64)):
+        raise ValueError(f"{name}: a row's heads and dims must be contiguous")
+    return t.data_ptr(), (t.stride(0) if rows > 1 else heads * 64)
+
+
+def _vec(t, dtype, name, device, numel=None):
+    """Address of a contiguous operand on `device` (None passes through)."""
+    if t is None:
+        return None
+    p = _dev(t, dtype, name)
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, not on {device}")
+    if numel is not None and t.numel() != numel:
+        raise ValueError(f"{name} must have {numel} elements, got {t.numel()}")
+    return p
+
+
+def _pages(page_table, pool, page_bytes, layer, device):
+    """The cache arguments of the C entry points from the page table [slots, max_pages] on."""
+    table = _vec(page_table, torch.int32, "page_table", device)
+    if page_table.dim() != 2:
+        raise ValueError("page_table must be [slots, max_pages]")
+    bytes_ = _vec(pool, torch.uint8, "pool", device)
+    if page_bytes <= 0:
+        raise ValueError(f"page_bytes {page_bytes}")
+    slots, max_pages = page_table.shape
+    return table, slots, max_pages, bytes_, page_bytes, pool.numel() // page_bytes, layer
+
+
+def _call_on(device, name, *args):
+    """The call on the device's current stream (whichever device is current)."""
+    if device.index == torch.cuda.current_device():
+        return call(name, *args, _stream())
+    with torch.cuda.device(device):
+        return call(name, *args, _stream())
+
+
+def kv_append(k, v, row_slot, row_pos, page_table, pool, page_bytes, layer, status=None):
+    """Rows of keys and values into the pages (ndl_kv_append).
+
+    k, v [rows, kv_heads, 64] of one type (float32, float16, bfloat16), rows
+    possibly strided; row_slot, row_pos int32 [rows] (distinct positions; a
+    negative position: padding); page_table int32 [slots, max_pages], pool
+    uint8 [num_pages * page_bytes]."""
+    code, device = _type(k, "k"), k.device
+    kp, ks = _heads(k, k.dtype, "k", device)
+    vp, vs = _heads(v, k.dtype, "v", device, k.shape)
+    rows, kv_heads, _ = k.shape
+    _call_on(device, "ndl_kv_append", kp, ks, vp, vs, code, _vec(row_slot, torch.int32, "row_slot", device, rows),
+             _vec(row_pos, torch.int32, "row_pos", device, rows), rows, kv_heads,
+             *_pages(page_table, pool, page_bytes, layer, device), _vec(status, torch.int32, "status", device))
+
+
+def kv_gather(row_slot, row_pos, kv_heads, page_table, pool, page_bytes, layer, dtype=torch.float32, k=None, v=None,
+              status=None):
+    """The values the pages hold for the rows (ndl_kv_gather): k and v
+    [rows, kv_heads, 64] of `dtype` (or of the tensors given)."""
+    device, rows = pool.device, row_slot.numel()
+    k = torch.empty((rows, kv_heads, 64), dtype=dtype, device=device) if k is None else k
+    v = torch.empty((rows, kv_heads, 64), dtype=k.dtype, device=device) if v is None else v
+    code = _type(k, "k")
+    kp, ks = _heads(k, k.dtype, "k", device, (rows, kv_heads, 64))
+    vp, vs = _heads(v, k.dtype, "v", device, (rows, kv_heads, 64))
+    _call_on(device, "ndl_kv_gather", _vec(row_slot, torch.int32, "row_slot", device),
+             _vec(row_pos, torch.int32, "row_pos", device, rows), rows, kv_heads,
+             *_pages(page_table, pool, page_bytes, layer, device), kp, ks, vp, vs, code,
+             _vec(status, torch.int32, "status", device))
+    return k, v
+
+
+def attention_prompt(q, seq_rows, seq_slot, seq_pos, kv_heads, page_table, pool, page_bytes, layer, scale=0.125,
+                     window=0, out=None, status=None):
+    """Whole-prompt causal attention over the pages (ndl_attention_prompt).
+
+    q [rows, heads, 64] (float32, float16, bfloat16; rows possibly strided)
+    packs the sequences: rows seq_rows[s] .. seq_rows[s+1] (int32
+    [sequences + 1]) are queries at positions seq_pos[s], seq_pos[s] + 1, ...
+    of slot seq_slot[s], whose pages hold the keys and values up to the last
+    of them.  window > 0: the last `window` positions only.  Rows of no
+    sequence are left as they are in `out`."""
+    code, device = _type(q, "q"), q.device
+    qp, qs = _heads(q, q.dtype, "q", device)
+    out = torch.empty(q.shape, dtype=q.dtype, device=device) if out is None else out
+    op, os_ = _heads(out, q.dtype, "out", device, q.shape)
+    rows, heads, _ = q.shape
+    sequences = seq_slot.numel()
+    _call_on(device, "ndl_attention_prompt", qp, qs, code,
+             _vec(seq_rows, torch.int32, "seq_rows", device, sequences + 1),
+             _vec(seq_slot, torch.int32, "seq_slot", device), _vec(seq_pos, torch.int32, "seq_pos", device, sequences),
+             sequences, rows, heads, kv_heads, scale, window, *_pages(page_table, pool, page_bytes, layer, device), op,
+             os_, _vec(status, torch.int32, "status", device))
+    return out
+
+
+def attention_split_workspace(rows, heads, kv_heads, max_pages):
+    return lib().ndl_attention_split_workspace(rows, heads, kv_heads, max_pages)
+
+
+def attention_split(q, row_slot, row_len, kv_heads, page_table, pool, page_bytes, layer, scale=0.125, window=0,
+                    out=None, workspace=None, status=None):
+    """Attention of single tokens, each split over its cache (ndl_attention_split).
+
+    q [rows, heads, 64] (float32, float16, bfloat16; rows possibly strided);
+    row r attends to the first row_len[r] positions (with window > 0 the last
+    `window` of them) of slot row_slot[r]; length 0 gives zeros.  workspace
+    uint8 [attention_split_workspace(...)]: allocated for the call if none is
+    given; calls that overlap need one each."""
+    code, device = _type(q, "q"), q.device
+    qp, qs = _heads(q, q.dtype, "q", device)
+    out = torch.empty(q.shape, dtype=q.dtype, device=device) if out is None else out
+    op, os_ = _heads(out, q.dtype, "out", device, q.shape)
+    rows, heads, _ = q.shape
+    pages = _pages(page_table, pool, page_bytes, layer, device)
+    if workspace is None:
+        need = lib().ndl_attention_split_workspace(rows, heads, kv_heads, pages[2])
+        workspace = torch.empty(need, dtype=torch.uint8, device=device)
+    _call_on(device, "ndl_attention_split", qp, qs, code, _vec(row_slot, torch.int32, "row_slot", device, rows),
+             _vec(row_len, torch.int32, "row_len", device, rows), rows, heads, kv_heads, scale, window, *pages, op, os_,
+             _vec(workspace, torch.uint8, "workspace", device), workspace.numel(),
+             _vec(status, torch.int32, "status", device))
+    return out
+
+
+def logits_process(logits, out=None, tokens=None, token_offsets=None, prompt_lens=None, repetition=None,
+                   frequency=None, presence=None, bias_ids=None, bias_values=None, bias_offsets=None, mask=None,
+                   mask_index=None, status=None):
+    """Penalties, biases and masks on logits [rows, vocab] fp32 (ndl_logits_process).
+
+    Row r's tokens are tokens[token_offsets[r]:token_offsets[r+1]] (int32), of
+    which the first prompt_lens[r] are the prompt; repetition, frequency,
+    presence fp32 [rows]; its biases bias_ids / bias_values
+    [bias_offsets[r]:bias_offsets[r+1]]; mask int32 [mask rows, words] (bit
+    set: allowed), row mask_index[r] of it (negative: none), without
+    mask_index row r.  out may be `logits` itself."""
+    device = logits.device
+    if logits.dim() != 2:
+        raise ValueError("logits must be [rows, vocab]")
+    rows, vocab = logits.shape
+    out = torch.empty((rows, vocab), dtype=torch.float32, device=device) if out is None else out
+
+    def matrix(t, name):
+        if not t.is_cuda or t.dtype != torch.float32:
+            raise TypeError(f"{name} must be a float32 CUDA tensor")
+        if t.device != device or tuple(t.shape) != (rows, vocab) or (vocab > 1 and t.stride(1) != 1):
+            raise ValueError(f"{name} must be [{rows}, {vocab}] on {device} with contiguous rows")
+        return t.data_ptr(), (t.stride(0) if rows > 1 else vocab)
+
+    i32, f32 = torch.int32, torch.float32
+    mask_rows, words = (0, 0) if mask is None else mask.shape
+    _call_on(device, "ndl_logits_process", *matrix(logits, "logits"), *matrix(out, "out"), rows, vocab,
+             _vec(tokens, i32, "tokens", device), 0 if tokens is None else tokens.numel(),
+             _vec(token_offsets, i32, "token_offsets", device, rows + 1),
+             _vec(prompt_lens, i32, "prompt_lens", device, rows), _vec(repetition, f32, "repetition", device, rows),
+             _vec(frequency, f32, "frequency", device, rows), _vec(presence, f32, "presence", device, rows),
+             _vec(bias_ids, i32, "bias_ids", device),
+             _vec(bias_values, f32, "bias_values", device, None if bias_ids is None else bias_ids.numel()),
+             0 if bias_ids is None else bias_ids.numel(), _vec(bias_offsets, i32, "bias_offsets", device, rows + 1),
+             _vec(mask, i32, "mask", device), mask_rows, words, _vec(mask_index, i32, "mask_index", device, rows),
+             _vec(status, i32, "status", device))
+    return out
