@@ -251,7 +251,7 @@ NDL_API int ndl_kv_gather(const int32_t *row_slot, const int32_t *row_pos, int r
  * probabilities to fp16 before the second product, fp32 splits queries and
  * probabilities into two fp16 parts.  Rows of no sequence are left as they
  * are; a sequence whose offsets descend or leave [0, rows] is skipped with
- * status 2. */
+ * status 2, and so may be those behind it. */
 NDL_API int ndl_attention_prompt(const void *q, long long q_stride, int type, const int32_t *seq_rows,
                                  const int32_t *seq_slot, const int32_t *seq_pos, int sequences, int rows, int heads,
                                  int kv_heads, float scale, int window, const int32_t *page_table, int slots,
