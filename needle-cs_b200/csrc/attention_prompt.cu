@@ -22,7 +22,7 @@
 // exchange), 4 that convert pages (int8 in global memory -> fp16 tiles in
 // shared memory, 128-byte swizzled rows), 1 that issues every MMA.  P goes
 // back to TMEM, from where the second product takes it as its A operand.
-#include "attention_row.cuh"
+#include "attention_math.cuh"
 #include "tc.cuh"
 
 namespace ndl {
@@ -40,8 +40,6 @@ constexpr uint32_t kPromptWait = 1u << 22;     // waits of about a microsecond: 
 // TMEM columns: scores, outputs, probabilities (two fp16 a column) of both tiles
 constexpr int kColS = 0, kColO = 128, kColP = 256, kColLo = 64;
 constexpr int kTmemCols = 512;
-constexpr float kLazy = 7.0f;
-constexpr int kMinExp = -110;                  // value scales below 2^-110 do not move k
 
 struct PromptArgs {
     const void *q;
@@ -95,60 +93,6 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32
         : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ float exp2_approx(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-// 2^e as a float, -126 <= e <= 127.
-__device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }
-
-// Four int8 codes of a word as two pairs of fp16, exactly: the biased byte in
-// the low mantissa bits of 1024, less 1024 + 128.
-__device__ __forceinline__ void codes_to_half(uint32_t w, uint32_t &lo, uint32_t &hi) {
-    const uint32_t u = w ^ 0x80808080u;
-    const __half2 bias = __half2half2(__ushort_as_half(0x6480));  // 1152
-    __half2 a, b;
-    *reinterpret_cast<uint32_t *>(&a) = __byte_perm(u, 0x64646464u, 0x4140);
-    *reinterpret_cast<uint32_t *>(&b) = __byte_perm(u, 0x64646464u, 0x4342);
-    a = __hsub2(a, bias), b = __hsub2(b, bias);
-    lo = *reinterpret_cast<uint32_t *>(&a), hi = *reinterpret_cast<uint32_t *>(&b);
-}
-__device__ __forceinline__ uint32_t half_pair(float a, float b) {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t *>(&h);
-}
-// The remainders of a pair behind its fp16 rounding.
-__device__ __forceinline__ uint32_t half_rest(float a, float b, uint32_t pair) {
-    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&pair));
-    return half_pair(a - f.x, b - f.y);
-}
-
-// Eight elements of a query row from element i on (i a multiple of 4 for fp32).
-template <class T>
-__device__ __forceinline__ void load4(const T *p, float (&x)[4]) {
-    if constexpr (sizeof(T) == 4) {
-        const float4 v = *reinterpret_cast<const float4 *>(p);
-        x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
-    } else {
-        const uint2 v = *reinterpret_cast<const uint2 *>(p);
-        const T *h = reinterpret_cast<const T *>(&v);
-#pragma unroll
-        for (int i = 0; i < 4; i++) x[i] = to_float(h[i]);
-    }
-}
-template <class T>
-__device__ __forceinline__ void store16(T *p, const float *x) {  // 16 bytes: 4 or 8 elements
-    if constexpr (sizeof(T) == 4) {
-        *reinterpret_cast<float4 *>(p) = make_float4(x[0], x[1], x[2], x[3]);
-    } else {
-        alignas(16) T h[8];
-#pragma unroll
-        for (int i = 0; i < 8; i++) h[i] = from_float<T>(x[i]);
-        *reinterpret_cast<uint4 *>(p) = *reinterpret_cast<const uint4 *>(h);
-    }
-}
-
 template <class T, bool kSplit>
 __global__ void __launch_bounds__(kPromptThreads, 1) attention_prompt_kernel(PromptArgs a) {
     extern __shared__ uint8_t smem_raw[];
@@ -249,10 +193,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attention_prompt_kernel(Pro
 #pragma unroll
                 for (int j = 0; j < 4; j++) x[i + j] = f[j], peak = fmaxf(peak, fabsf(f[j]));
             }
-            int e = (int)((__float_as_uint(peak) >> 23) & 0xFF) - 127;
-            e = e == 128 ? 10 : max(e, -100);  // an infinity stays one
-            const float up = pow2(10 - e);
-            scale_q = pow2(e - 10);
+            float up;
+            query_norm(peak, up, scale_q);
 #pragma unroll
             for (int j = 0; j < 8; j++) {  // 16-byte chunk j: dims d..d+3 and d+16..d+19
                 const int d = (j >> 2) * 32 + (j & 3) * 4;
@@ -274,7 +216,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attention_prompt_kernel(Pro
         const uint32_t ts = tmem + lanes + kColS + t * 64, to = tmem + lanes + kColO + t * 64;
         const uint32_t tp = tmem + lanes + kColP + t * 32;
         float top = -INFINITY, total = 0.0f;
-        int exponent = kMinExp;
+        int exponent = kMinExponent;
         bool ok = true;
         for (int i = lo[t]; i <= hi[t]; i++) {
             const int it = i - lo[t], st = (i - page0) % kStages;
@@ -409,14 +351,14 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attention_prompt_kernel(Pro
     } else if (warp < kMmaWarp) {
         // -------------------------------------------------- page converter --
         const int c = warp - kConvertWarp;
-        int exponent = kMinExp;
+        int exponent = kMinExponent;
         int ids = 0;
         struct Page {
             uint4 k[2], v[2];
             float2 scale;
             int id;
         } cur, nxt;
-        const float fold = a.scale * 1.44269504088896341f;
+        const float fold = a.scale * kLog2E;
         auto fetch = [&](int i, Page &p) {
             const int rel = i - page0;
             if ((rel & 31) == 0) ids = i + lane <= page1 ? cache_page(a.c, slot, i + lane) : -1;
@@ -489,11 +431,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attention_prompt_kernel(Pro
                 s.ks[st][lane + 32] = f.y * fold;
             } else if (c == 1) {
                 if (!there) f.x = f.y = 0.0f;
-                int e = max((int)((__float_as_uint(f.x) >> 23) & 0xFF), 0);
-                int e2 = (int)((__float_as_uint(f.y) >> 23) & 0xFF);
-                e = e == 255 ? 0 : e, e2 = e2 == 255 ? 0 : e2;
-                e = __reduce_max_sync(0xffffffffu, max(e, e2)) - 126;  // below 2^e
-                exponent = max(exponent, e);
+                const int e = __reduce_max_sync(0xffffffffu, max(scale_exponent(f.x), scale_exponent(f.y)));
+                exponent = max(exponent, e - 126);
                 const float down = pow2(8 - exponent);  // -110 <= exponent <= 128
                 s.vs[st][lane] = f.x * down;
                 s.vs[st][lane + 32] = f.y * down;

@@ -1,43 +1,576 @@
-// Attention of single tokens over the paged int8 cache.
-#include "attention_row.cuh"
+// Attention of single tokens over the paged int8 cache, split over its length.
+//
+// A row's query heads that share a kv head (at most 16 at a time) attend
+// together; such an item reads one 8704-byte record per page.  All records of
+// a call, item after item, are dealt out evenly: worker w of W (a warp) takes
+// records [T w / W, T (w + 1) / W), whatever the rows' lengths are, so one
+// long row fills the card as well as many ragged ones.  A worker streams its
+// records through its own ring in shared memory (one bulk copy each, 8 warps
+// x 3 records = 209 KB in flight an SM against the ~45 KB that bandwidth times
+// latency asks for) and keeps a running maximum, sum and output per head:
+//   S = Q K^T, O += (e vs) V   mma.sync m16n8k16 (heads x positions / dims);
+// the codes become fp16 exactly in registers, from the fragments the pages
+// hold.  Tensor cores because a position costs 128 products a head and 128
+// conversions, and a kv head's group shares the conversions; tcgen05 would
+// need tiles of 128 rows, and there are at most 16.
+// An item inside one worker is finished there; pieces of the others (O / l,
+// m, l) go to the workspace, and a second kernel, launched early, joins them
+// in order, so the result does not depend on timing.
+//
+// Number ranges as in attention_prompt.cu: queries normalised per row by a
+// power of two, value scales by that of the largest so far, the maximum
+// followed lazily; fp32 splits queries and probabilities in two fp16 parts.
+#include <float.h>
+
+#include "attention_math.cuh"
 
 namespace ndl {
+
+namespace {
+
+constexpr int kSplitWarps = 8, kSplitThreads = 32 * kSplitWarps, kSplitStages = 3;
+constexpr int kSplitCtas = 148;                       // one CTA an SM
+constexpr int kSplitWorkers = kSplitCtas * kSplitWarps;
+constexpr int kHeadBlock = 16;                        // query heads an item holds
+constexpr uint32_t kSplitWait = 1u << 22;             // tests of about a microsecond: a few seconds
+// A piece: per head 64 outputs, m and l (padded to 16 bytes).
+constexpr int kPieceHead = 68;
+constexpr int kJoinThreads = 256;
 
 struct SplitArgs {
     const void *q;
     void *out;
     long long q_stride, out_stride;
     const int32_t *row_slot, *row_len;
-    int rows, heads, window;
+    int rows, heads, group, blocks, window;  // blocks: items a kv head and row
+    int piece_heads;                         // heads a piece holds: min(group, 16)
     float scale;
     PagedCache c;
+    long long *prefix;  // [rows + 1]: records before each row
+    float *pieces;      // [kSplitWorkers][2][piece_heads][kPieceHead]
 };
 
-template <class T>
-__global__ void __launch_bounds__(128) attention_split_kernel(SplitArgs a) {
-    __shared__ float q[4][64];
-    const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const long long item = (long long)blockIdx.x * 4 + w;
-    if (item >= (long long)a.rows * a.heads) return;
-    const int row = (int)(item / a.heads), head = (int)(item % a.heads);
-    const T *src = static_cast<const T *>(a.q) + (size_t)row * a.q_stride + head * 64;
-    q[w][lane] = to_float(src[lane]) * a.scale;
-    q[w][lane + 32] = to_float(src[lane + 32]) * a.scale;
-    __syncwarp();
+// Pages [first, last) that a row reads (none for an empty or a bad row).
+__device__ __forceinline__ bool row_pages(const SplitArgs &a, int row, int &first, int &last) {
     const int slot = a.row_slot[row], len = a.row_len[row];
-    bool ok = slot >= 0 && slot < a.c.slots && len >= 0 && len <= a.c.max_pages * 64;
-    float o0, o1;
-    if (ok)
-        ok = attend_row(a.c, slot, head / (a.heads / a.c.heads), a.window ? max(0, len - a.window) : 0, len, q[w], o0,
-                        o1, lane);
-    if (!ok) {
-        if (lane == 0 && a.c.status) atomicOr(a.c.status, kStatusBadPage);
-        o0 = o1 = __int_as_float(0x7fc00000);
-    }
-    T *dst = static_cast<T *>(a.out) + (size_t)row * a.out_stride + head * 64;
-    dst[lane] = from_float<T>(o0);
-    dst[lane + 32] = from_float<T>(o1);
+    first = last = 0;
+    if (slot < 0 || slot >= a.c.slots || len < 0 || len > a.c.max_pages * kPagePositions) return false;
+    if (len == 0) return true;
+    first = (a.window ? max(0, len - a.window) : 0) / kPagePositions;
+    last = (len - 1) / kPagePositions + 1;
+    return true;
 }
+__device__ __forceinline__ int worker_count(long long records) {
+    return records < kSplitWorkers ? (int)records : kSplitWorkers;
+}
+__device__ __forceinline__ long long worker_start(long long records, int workers, int w) {
+    return records * w / workers;
+}
+
+struct SplitSmem {
+    uint8_t ring[kSplitWarps][kSplitStages][kKvBlockBytes];
+    uint64_t full[kSplitWarps][kSplitStages];
+    long long sums[kSplitThreads + 1];
+};
+
+// Where a worker stands: item (row, virtual head) and page of it.
+struct SplitCursor {
+    int row, item, page, first, last;
+};
+
+// The state of one item's heads: outputs (8 dim blocks), maximum, sum.
+template <bool kWide>
+struct SplitState {
+    static constexpr int kRows = kWide ? 2 : 1;  // heads lane / 4 and, wide, lane / 4 + 8
+    float o[8][4];
+    float top[kRows], total[kRows];
+    int exponent;
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int d = 0; d < 8; d++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) o[d][i] = 0.0f;
+#pragma unroll
+        for (int r = 0; r < kRows; r++) top[r] = -INFINITY, total[r] = 0.0f;
+        exponent = kMinExponent;
+    }
+};
+
+// The query fragments of an item: k-step (s, h) covers dims 32 s + 16 h + 4 t
+// .. + 3 of lane t = lane & 3 (as the key fragments hold them).
+template <bool kWide, bool kSplit>
+struct SplitQuery {
+    static constexpr int kRows = kWide ? 2 : 1;
+    uint32_t a[kSplit ? 2 : 1][4][kRows][2];  // [part][k-step][head half][dim pair]
+    float factor[kRows];                      // scores -> binary orders
+};
+
+template <class T, bool kWide, bool kSplit>
+__device__ __forceinline__ void load_query(const SplitArgs &a, int row, int item, int lane,
+                                           SplitQuery<kWide, kSplit> &q) {
+    const int kv = item / a.blocks, block = item - kv * a.blocks;
+#pragma unroll
+    for (int r = 0; r < (kWide ? 2 : 1); r++) {
+        const int in_group = block * kHeadBlock + r * 8 + (lane >> 2);
+        const bool there = in_group < a.group;
+        const T *src = static_cast<const T *>(a.q) + (size_t)row * a.q_stride +
+                       ((size_t)kv * a.group + (there ? in_group : 0)) * kHeadDim + (lane & 3) * 4;
+        float x[4][4], peak = 0.0f;
+#pragma unroll
+        for (int s = 0; s < 4; s++) {
+            load4(src + 16 * s, x[s]);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                if (!there) x[s][i] = 0.0f;
+                peak = fmaxf(peak, fabsf(x[s][i]));
+            }
+        }
+        peak = fmaxf(peak, __shfl_xor_sync(0xffffffffu, peak, 1));
+        peak = fmaxf(peak, __shfl_xor_sync(0xffffffffu, peak, 2));
+        float up, down;
+        query_norm(peak, up, down);
+        q.factor[r] = fmaxf(down * a.scale * kLog2E, FLT_MIN);  // not zero: it multiplies infinities
+#pragma unroll
+        for (int s = 0; s < 4; s++)
+#pragma unroll
+            for (int p = 0; p < 2; p++) {
+                const float f0 = x[s][2 * p] * up, f1 = x[s][2 * p + 1] * up;
+                q.a[0][s][r][p] = half_pair(f0, f1);
+                if constexpr (kSplit) q.a[kSplit ? 1 : 0][s][r][p] = half_rest(f0, f1, q.a[0][s][r][p]);
+            }
+    }
+}
+
+__device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                          uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+
+// One page into the state.  Positions [from, upto) of it count.
+template <bool kWide, bool kSplit>
+__device__ __forceinline__ void attend_page(const uint8_t *rec, int from, int upto, int lane,
+                                            const SplitQuery<kWide, kSplit> &q, SplitState<kWide> &st) {
+    constexpr int R = kWide ? 2 : 1;
+    const int t = lane & 3;
+    // scores: n-tile (T, h) holds positions 16 T + 8 h + 0..7, this lane's 2 t and 2 t + 1
+    float s[4][2][4];
+#pragma unroll
+    for (int T = 0; T < 4; T++) {
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) s[T][h][i] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            const uint4 w = *reinterpret_cast<const uint4 *>(rec + T * 1024 + k * 512 + lane * 16);
+            const uint32_t words[4] = {w.x, w.y, w.z, w.w};  // (row, dims), (row + 8, dims), dims + 16 likewise
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                uint32_t b0, b1;
+                codes_to_half(words[u], b0, b1);
+                const int ks = 2 * k + (u >> 1);
+#pragma unroll
+                for (int part = 0; part < (kSplit ? 2 : 1); part++)
+                    mma_16816(s[T][u & 1], q.a[part][ks][0][0], kWide ? q.a[part][ks][R - 1][0] : 0u,
+                              q.a[part][ks][0][1], kWide ? q.a[part][ks][R - 1][1] : 0u, b0, b1);
+            }
+        }
+    }
+    // key scales of positions 2 t + e: eight (T, h) in a row
+    const float4 *ks = reinterpret_cast<const float4 *>(rec + kKScaleOffset) + 4 * t;
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+        const float4 c0 = ks[2 * e], c1 = ks[2 * e + 1];
+        const float c[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
+#pragma unroll
+        for (int T = 0; T < 4; T++)
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+                for (int r = 0; r < R; r++) s[T][h][2 * r + e] *= c[2 * T + h];
+    }
+    const bool whole = from <= 0 && upto >= kPagePositions;
+    if (!whole) {
+#pragma unroll
+        for (int T = 0; T < 4; T++)
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const int p = 16 * T + 8 * h + 2 * t + e;
+                    if (p < from || p >= upto)
+#pragma unroll
+                        for (int r = 0; r < R; r++) s[T][h][2 * r + e] = -INFINITY;
+                }
+    }
+    // value scales over 2^exponent (of the largest so far) times 2^8
+    float2 vs[4][2];
+    int big = 0;
+#pragma unroll
+    for (int T = 0; T < 4; T++)
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            float2 v = *reinterpret_cast<const float2 *>(rec + kVScaleOffset + (16 * T + 8 * h + 2 * t) * 4);
+            if (!whole) {
+                const int p = 16 * T + 8 * h + 2 * t;
+                if (p < from || p >= upto) v.x = 0.0f;
+                if (p + 1 < from || p + 1 >= upto) v.y = 0.0f;
+            }
+            vs[T][h] = v;
+            big = max(big, max(scale_exponent(v.x), scale_exponent(v.y)));
+        }
+    const int exponent = max(st.exponent, __reduce_max_sync(0xffffffffu, big) - 126);
+    const float norm = pow2(8 - exponent);
+    float keep[R], base[R];
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        float peak = -INFINITY;
+#pragma unroll
+        for (int T = 0; T < 4; T++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) peak = fmaxf(peak, fmaxf(s[T][h][2 * r], s[T][h][2 * r + 1]));
+        peak = fmaxf(peak, __shfl_xor_sync(0xffffffffu, peak, 1));
+        peak = fmaxf(peak, __shfl_xor_sync(0xffffffffu, peak, 2));
+        keep[r] = exponent > st.exponent ? exp2_approx((float)(st.exponent - exponent)) : 1.0f;
+        if ((peak - st.top[r]) * q.factor[r] > kLazy || (st.top[r] == -INFINITY && peak > -INFINITY)) {
+            const float k = st.top[r] == -INFINITY ? 0.0f : exp2_approx((st.top[r] - peak) * q.factor[r]);
+            st.total[r] *= k, keep[r] *= k;
+            st.top[r] = peak;
+        }
+        base[r] = st.top[r] == -INFINITY ? 0.0f : st.top[r] * q.factor[r];
+    }
+    st.exponent = exponent;
+    bool moved = keep[0] != 1.0f;
+    if constexpr (kWide) moved = moved || keep[R - 1] != 1.0f;
+    if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+        for (int d = 0; d < 8; d++)
+#pragma unroll
+            for (int r = 0; r < R; r++) st.o[d][2 * r] *= keep[r], st.o[d][2 * r + 1] *= keep[r];
+    }
+    // probabilities: the second product's k-step T wants positions 4 t .. 4 t + 3 of 16 in lane t (as ldmatrix hands
+    // out the value bytes), the scores left 2 t, 2 t + 1 and 8 + 2 t, 9 + 2 t there
+    uint32_t p[kSplit ? 2 : 1][4][R][2];
+    const int src = (lane & ~3) | ((2 * t) & 3);
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int T = 0; T < 4; T++) {
+            uint32_t hi[2], lo[2] = {0, 0};
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const float e0 = exp2_approx(fmaf(s[T][h][2 * r], q.factor[r], -base[r]));
+                const float e1 = exp2_approx(fmaf(s[T][h][2 * r + 1], q.factor[r], -base[r]));
+                sum += e0 + e1;
+                float p0 = e0 * (vs[T][h].x * norm), p1 = e1 * (vs[T][h].y * norm);
+                hi[h] = half_pair(p0, p1);
+                if constexpr (kSplit) lo[h] = half_rest(p0, p1, hi[h]);
+            }
+#pragma unroll
+            for (int part = 0; part < (kSplit ? 2 : 1); part++) {
+                const uint32_t *x = part ? lo : hi;
+                const uint32_t a0 = __shfl_sync(0xffffffffu, x[0], src), b0 = __shfl_sync(0xffffffffu, x[1], src);
+                const uint32_t a1 = __shfl_sync(0xffffffffu, x[0], src + 1);
+                const uint32_t b1 = __shfl_sync(0xffffffffu, x[1], src + 1);
+                p[part][T][r][0] = t < 2 ? a0 : b0;
+                p[part][T][r][1] = t < 2 ? a1 : b1;
+            }
+        }
+        st.total[r] += sum;
+    }
+    // O += P V: dims 8 D + (lane >> 2)
+    const int d8 = lane & 7, T4 = lane >> 3;
+#pragma unroll
+    for (int D = 0; D < 8; D++) {
+        const int d = 8 * D + d8;
+        uint32_t w[4];
+        ldmatrix4(w, smem_u32(rec + kVOffset + d * 64 + ((T4 ^ ((d >> 1) & 3)) << 4)));
+#pragma unroll
+        for (int T = 0; T < 4; T++) {
+            uint32_t b0, b1;
+            codes_to_half(w[T], b0, b1);
+#pragma unroll
+            for (int part = 0; part < (kSplit ? 2 : 1); part++)
+                mma_16816(st.o[D], p[part][T][0][0], kWide ? p[part][T][R - 1][0] : 0u, p[part][T][0][1],
+                          kWide ? p[part][T][R - 1][1] : 0u, b0, b1);
+        }
+    }
+}
+
+template <class T, bool kWide>
+__global__ void __launch_bounds__(kSplitThreads, 1) attention_split_kernel(SplitArgs a) {
+    constexpr bool kSplit = sizeof(T) == 4;
+    constexpr int R = kWide ? 2 : 1;
+    extern __shared__ uint8_t smem_raw[];
+    SplitSmem &s = *reinterpret_cast<SplitSmem *>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~uintptr_t(127));
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int virtual_heads = a.c.heads * a.blocks;
+    pdl_trigger();  // the joining kernel waits for this one's end by itself
+
+    // Records before each row: a thread sums a run of rows, the CTA scans the runs.
+    const int run = (a.rows + kSplitThreads - 1) / kSplitThreads;
+    {
+        long long mine = 0;
+        for (int i = threadIdx.x * run; i < min(a.rows, (int)(threadIdx.x + 1) * run); i++) {
+            int first, last;
+            row_pages(a, i, first, last);
+            mine += (long long)(last - first) * virtual_heads;
+        }
+        long long sum = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long up = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += up;
+        }
+        if (lane == 31) s.sums[warp + 1] = sum;
+        if (threadIdx.x < kSplitWarps * kSplitStages) mbar_init(&s.full[0][0] + threadIdx.x, 1);
+        fence_mbar_init();
+        __syncthreads();
+        long long before = 0;
+        for (int w = 0; w < warp; w++) before += s.sums[w + 1];
+        __syncthreads();
+        s.sums[threadIdx.x + 1] = before + sum;
+        if (threadIdx.x == 0) s.sums[0] = 0;
+        __syncthreads();
+        if (blockIdx.x == 0) {
+            long long at = before + sum - mine;
+            for (int i = threadIdx.x * run; i < min(a.rows, (int)(threadIdx.x + 1) * run); i++) {
+                int first, last;
+                row_pages(a, i, first, last);
+                a.prefix[i] = at;
+                at += (long long)(last - first) * virtual_heads;
+            }
+            if (threadIdx.x == 0) a.prefix[a.rows] = s.sums[kSplitThreads];
+        }
+    }
+    const long long records = s.sums[kSplitThreads];
+    const int workers = worker_count(records);
+    const int worker = warp * gridDim.x + blockIdx.x;  // the first workers sit on different SMs
+    if (worker >= workers) return;
+    const long long begin = worker_start(records, workers, worker), end = worker_start(records, workers, worker + 1);
+
+    // the first record's row, item and page
+    SplitCursor cur;
+    long long item_at;  // record index of the current item's first page
+    {
+        int lo = 0, hi = kSplitThreads;  // the run: sums[lo] <= begin < sums[hi]
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (s.sums[mid] <= begin) lo = mid;
+            else hi = mid;
+        }
+        long long at = s.sums[lo];
+        int row = lo * run;
+        for (;; row++) {
+            row_pages(a, row, cur.first, cur.last);
+            const long long n = (long long)(cur.last - cur.first) * virtual_heads;
+            if (begin < at + n) break;
+            at += n;
+        }
+        const int pages = cur.last - cur.first;
+        cur.row = row;
+        cur.item = (int)((begin - at) / pages);
+        cur.page = cur.first + (int)((begin - at) % pages);
+        item_at = at + (long long)cur.item * pages;
+    }
+    // the copies' own place, ahead of the reading
+    SplitCursor ahead = cur;
+    int ids = -1, ids_row = -1, ids_at = -1, slot = 0;
+    uint32_t bad = 0;  // ring stages whose page is missing
+    long long next = begin;
+    auto issue = [&](int stage) {  // the copy of record `next`
+        const int at = ahead.page & ~31;
+        if (ahead.row != ids_row || at != ids_at) {
+            ids_row = ahead.row, ids_at = at;
+            slot = a.row_slot[ahead.row];
+            ids = at + lane < ahead.last ? cache_page(a.c, slot, at + lane) : -1;
+        }
+        const int page = __shfl_sync(0xffffffffu, ids, ahead.page & 31);
+        bad = page < 0 ? bad | (1u << stage) : bad & ~(1u << stage);
+        if (page >= 0 && lane == 0) {
+            mbar_arrive_expect_tx(&s.full[warp][stage], kKvBlockBytes);
+            bulk_g2s(s.ring[warp][stage], cache_record(a.c, page, ahead.item / a.blocks), kKvBlockBytes,
+                     &s.full[warp][stage]);
+        }
+        next++;
+        if (++ahead.page == ahead.last && next < end) {
+            if (++ahead.item == virtual_heads) {
+                ahead.item = 0;
+                do {
+                    ahead.row++;
+                    row_pages(a, ahead.row, ahead.first, ahead.last);
+                } while (ahead.first == ahead.last);
+            }
+            ahead.page = ahead.first;
+        }
+    };
+    for (int i = 0; i < kSplitStages && next < end; i++) issue(i);
+
+    SplitQuery<kWide, kSplit> q;
+    SplitState<kWide> st;
+    load_query<T, kWide, kSplit>(a, cur.row, cur.item, lane, q);
+    st.clear();
+    int len = a.row_len[cur.row];
+    int piece = 0;           // this worker's pieces: 0 starts at its first record, 1 is a later one
+    uint32_t phases = 0;     // parity of each stage's next completed copy
+    bool timed_out = false;
+    int stage = 0;
+    for (long long rec = begin; rec < end; rec++) {
+        if (bad >> stage & 1) {
+#pragma unroll
+            for (int r = 0; r < R; r++) st.total[r] = __int_as_float(0x7fc00000);
+            if (lane == 0 && a.c.status) atomicOr(a.c.status, kStatusBadPage);
+        } else {
+            const bool ok = mbar_wait_bounded(&s.full[warp][stage], phases >> stage & 1, kSplitWait);
+            if (!__all_sync(0xffffffffu, ok)) {
+                timed_out = true;
+                break;
+            }
+            phases ^= 1u << stage;
+            const int at = cur.page * kPagePositions;
+            attend_page<kWide, kSplit>(s.ring[warp][stage], a.window ? len - a.window - at : 0, len - at, lane, q, st);
+        }
+        __syncwarp();
+        if (next < end) issue(stage);
+        stage = stage + 1 == kSplitStages ? 0 : stage + 1;
+
+        const bool item_ends = cur.page + 1 == cur.last;
+        if (item_ends || rec + 1 == end) {
+            // the item, or this worker's piece of it
+            const bool alone = item_ends && item_at >= begin;
+            const int kv = cur.item / a.blocks, block = cur.item - kv * a.blocks;
+            const float back = pow2(st.exponent - 8);
+#pragma unroll
+            for (int r = 0; r < R; r++) {
+                float total = st.total[r];
+                total += __shfl_xor_sync(0xffffffffu, total, 1);
+                total += __shfl_xor_sync(0xffffffffu, total, 2);
+                const float inverse = 1.0f / total;
+                const int in_block = r * 8 + (lane >> 2), in_group = block * kHeadBlock + in_block;
+                if (in_group >= a.group) continue;
+                if (alone) {
+                    T *dst = static_cast<T *>(a.out) + (size_t)cur.row * a.out_stride +
+                             ((size_t)kv * a.group + in_group) * kHeadDim + 2 * (lane & 3);
+#pragma unroll
+                    for (int D = 0; D < 8; D++)
+                        store2(dst + 8 * D, st.o[D][2 * r] * inverse * back, st.o[D][2 * r + 1] * inverse * back);
+                } else {
+                    float *dst = a.pieces + (((size_t)worker * 2 + piece) * a.piece_heads + in_block) * kPieceHead;
+#pragma unroll
+                    for (int D = 0; D < 8; D++)
+                        *reinterpret_cast<float2 *>(dst + 8 * D + 2 * (lane & 3)) =
+                            make_float2(st.o[D][2 * r] * inverse * back, st.o[D][2 * r + 1] * inverse * back);
+                    if ((lane & 3) == 0)
+                        *reinterpret_cast<float2 *>(dst + kHeadDim) = make_float2(st.top[r] * q.factor[r], total);
+                }
+            }
+            if (rec + 1 < end) {
+                item_at = rec + 1;
+                piece = 1;
+                if (++cur.item == virtual_heads) {
+                    cur.item = 0;
+                    do {
+                        cur.row++;
+                        row_pages(a, cur.row, cur.first, cur.last);
+                    } while (cur.first == cur.last);
+                    len = a.row_len[cur.row];
+                }
+                cur.page = cur.first;
+                load_query<T, kWide, kSplit>(a, cur.row, cur.item, lane, q);
+                st.clear();
+            }
+        } else {
+            cur.page++;
+        }
+    }
+    if (timed_out) {
+        if (lane == 0 && a.c.status) atomicOr(a.c.status, kStatusTimeout);
+        // every copy in flight lands before the warp exits (bounded)
+        for (int i = 0; i < kSplitStages; i++)
+            if (!(bad >> i & 1)) mbar_wait_bounded(&s.full[warp][i], phases >> i & 1, kSplitWait);
+    }
+}
+
+// Joins the pieces of one item (CTA) in worker order:
+//   out = sum w_i o_i / sum w_i,  w_i = l_i 2^(m_i - max m)
+// and writes the rows that have no records.
+template <class T>
+__global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(SplitArgs a) {
+    __shared__ float acc[kJoinThreads / 32][kHeadDim], weight[kJoinThreads / 32], tops[kJoinThreads / 32];
+    pdl_wait();
+    const int virtual_heads = a.c.heads * a.blocks;
+    const int row = blockIdx.x / virtual_heads, item = blockIdx.x - row * virtual_heads;
+    const int kv = item / a.blocks, block = item - kv * a.blocks;
+    const int heads = min(kHeadBlock, a.group - block * kHeadBlock);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    T *out = static_cast<T *>(a.out) + (size_t)row * a.out_stride +
+             ((size_t)kv * a.group + block * kHeadBlock) * kHeadDim;
+    const long long before = a.prefix[row], records = a.prefix[a.rows];
+    const long long pages = (a.prefix[row + 1] - before) / virtual_heads;
+    if (pages == 0) {
+        int first, last;
+        const bool good = row_pages(a, row, first, last);
+        if (!good && threadIdx.x == 0 && a.c.status) atomicOr(a.c.status, kStatusBadPage);
+        for (int i = threadIdx.x; i < heads * kHeadDim; i += kJoinThreads)
+            out[i] = from_float<T>(good ? 0.0f : __int_as_float(0x7fc00000));
+        return;
+    }
+    const int workers = worker_count(records);
+    const long long begin = before + item * pages, end = begin + pages;
+    // the workers whose ranges hold its first and last record
+    auto holder = [&](long long rec) {
+        int w = (int)(((double)rec + 0.5) * workers / (double)records);
+        w = max(0, min(workers - 1, w));
+        while (worker_start(records, workers, w) > rec) w--;
+        while (worker_start(records, workers, w + 1) <= rec) w++;
+        return w;
+    };
+    const int w0 = holder(begin), w1 = holder(end - 1);
+    if (w0 == w1) return;  // that worker wrote it
+    const int first_piece = worker_start(records, workers, w0) == begin ? 0 : 1;
+    for (int h = 0; h < heads; h++) {
+        float top = -INFINITY, sum = 0.0f, o0 = 0.0f, o1 = 0.0f;
+        // a warp takes a run of the pieces, in order
+        const int count = w1 - w0 + 1, per = (count + kJoinThreads / 32 - 1) / (kJoinThreads / 32);
+        const int from = w0 + warp * per, to = min(w1 + 1, from + per);
+#pragma unroll 4
+        for (int w = from; w < to; w++) {
+            const float *p = a.pieces + (((size_t)w * 2 + (w == w0 ? first_piece : 0)) * a.piece_heads + h) * kPieceHead;
+            const float2 ml = *reinterpret_cast<const float2 *>(p + kHeadDim);
+            const float2 v = *reinterpret_cast<const float2 *>(p + 2 * lane);
+            const float m = fmaxf(top, ml.x);
+            const float keep = top == m ? 1.0f : exp2f(top - m), add = ml.x == m ? ml.y : ml.y * exp2f(ml.x - m);
+            sum = sum * keep + add, o0 = o0 * keep + add * v.x, o1 = o1 * keep + add * v.y;
+            top = m;
+        }
+        acc[warp][2 * lane] = o0, acc[warp][2 * lane + 1] = o1;
+        if (lane == 0) weight[warp] = sum, tops[warp] = top;
+        __syncthreads();
+        if (threadIdx.x < kHeadDim) {
+            float m = -INFINITY, w = 0.0f, o = 0.0f;
+            for (int i = 0; i < kJoinThreads / 32; i++) m = fmaxf(m, tops[i]);
+            for (int i = 0; i < kJoinThreads / 32; i++) {
+                if (tops[i] == -INFINITY && weight[i] == 0.0f) continue;  // no pieces
+                const float f = tops[i] == m ? 1.0f : exp2f(tops[i] - m);
+                w += weight[i] * f, o += acc[i][threadIdx.x] * f;
+            }
+            out[h * kHeadDim + threadIdx.x] = from_float<T>(o / w);
+        }
+        __syncthreads();
+    }
+}
+
+}  // namespace
 
 int check_attention(const void *q, long long q_stride, const void *out, long long out_stride, int type, int rows,
                     int heads, int kv_heads, float scale, int window) {
@@ -50,11 +583,18 @@ int check_attention(const void *q, long long q_stride, const void *out, long lon
     return rc == NDL_OK ? check_rows("out", out, type, heads, out_stride) : rc;
 }
 
+static size_t prefix_bytes(int rows) { return (((size_t)rows + 1) * sizeof(long long) + 15) & ~size_t(15); }
+
 }  // namespace ndl
 
 using namespace ndl;
 
-extern "C" NDL_API size_t ndl_attention_split_workspace(int rows, int heads, int kv_heads, int max_pages) { return 0; }
+// The records before each row, and two pieces a worker.
+extern "C" NDL_API size_t ndl_attention_split_workspace(int rows, int heads, int kv_heads, int max_pages) {
+    if (rows <= 0 || heads <= 0 || kv_heads <= 0 || max_pages <= 0 || heads % kv_heads != 0) return 0;
+    const int held = heads / kv_heads < kHeadBlock ? heads / kv_heads : kHeadBlock;
+    return prefix_bytes(rows) + (size_t)kSplitWorkers * 2 * held * kPieceHead * sizeof(float);
+}
 
 extern "C" NDL_API int ndl_attention_split(const void *q, long long q_stride, int type, const int32_t *row_slot,
                                            const int32_t *row_len, int rows, int heads, int kv_heads, float scale,
@@ -69,14 +609,35 @@ extern "C" NDL_API int ndl_attention_split(const void *q, long long q_stride, in
     rc = check_attention(q, q_stride, out, out_stride, type, rows, heads, kv_heads, scale, window);
     if (rc != NDL_OK) return rc;
     const size_t need = ndl_attention_split_workspace(rows, heads, kv_heads, max_pages);
-    NDL_REQUIRE(aligned(workspace, 16) && (need == 0 || (workspace && workspace_bytes >= need)),
-                "workspace of %zu bytes, %zu needed", workspace_bytes, need);
-    SplitArgs a{q, out, q_stride, out_stride, row_slot, row_len, rows, heads, window, scale,
+    NDL_REQUIRE(aligned(workspace, 16) && workspace && workspace_bytes >= need, "workspace of %zu bytes, %zu needed",
+                workspace_bytes, need);
+    const int group = heads / kv_heads;
+    SplitArgs a{q, out, q_stride, out_stride, row_slot, row_len, rows, heads, group,
+                (group + kHeadBlock - 1) / kHeadBlock, window, group < kHeadBlock ? group : kHeadBlock, scale,
                 {page_table, const_cast<uint8_t *>(pool), (long long)page_bytes, slots, max_pages, num_pages, layer,
-                 kv_heads, status}};
+                 kv_heads, status},
+                static_cast<long long *>(workspace),
+                reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + prefix_bytes(rows))};
     return with_type(type, [&](auto t) {
-        attention_split_kernel<decltype(t)>
-            <<<(unsigned)(((long long)rows * heads + 3) / 4), 128, 0, (cudaStream_t)stream>>>(a);
-        return check_launch("attention_split");
+        using T = decltype(t);
+        const auto kernel = group > 8 ? attention_split_kernel<T, true> : attention_split_kernel<T, false>;
+        constexpr size_t smem = sizeof(SplitSmem) + 128;
+        static DeviceOnce attribute;  // the attributes belong to the kernels on one device
+        const int st = attribute.run([&] {
+            for (const auto k : {attention_split_kernel<T, true>, attention_split_kernel<T, false>}) {
+                const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+                if (e != cudaSuccess)
+                    return set_error(NDL_ERR_CUDA, "split attention smem: %s", cudaGetErrorString(e));
+            }
+            return (int)NDL_OK;
+        });
+        if (st != NDL_OK) return st;
+        kernel<<<kSplitCtas, kSplitThreads, smem, (cudaStream_t)stream>>>(a);
+        const int rc2 = check_launch("attention_split");
+        if (rc2 != NDL_OK) return rc2;
+        PdlScope early(true);  // the join's launch overlaps the kernel above; it waits for its end before reading
+        launch_kernel(attention_join_kernel<T>, dim3((unsigned)(rows * kv_heads * a.blocks)), dim3(kJoinThreads), 0,
+                      (cudaStream_t)stream, a);
+        return check_launch("attention_join");
     });
 }
