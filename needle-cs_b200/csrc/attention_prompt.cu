@@ -4,24 +4,38 @@
 // A CTA takes 256 packed rows (two tiles of 128) of one sequence and kv head;
 // packed row m is query m / group of the sequence and query head m % group of
 // the kv head's group, so a page of keys and values serves every query head
-// that shares it.  It walks the pages its rows see, one page of 64 positions
-// a step, with the softmax's running maximum and sum:
+// that shares it.  It walks the pages its rows see, 128 positions a step
+// (fp32: 64), with the softmax's running maximum and sum:
 //   S = Q K^T       tcgen05.mma, fp16 operands, fp32 accumulator in TMEM
-//   t = S ks_j      (ks: the key scales, with scale * log2 e folded in)
-//   e = 2^(q (t - m)),  l += e,  P = e vs_j,  O += P V
-// q, a power of two per row, brings the row's largest query to [2^10, 2^11),
-// so 16-bit queries are exact in fp16; key and value codes are small integers,
-// exact too.  P rounds to fp16 (half a step, 2^-11, as an fp16 result does);
-// fp32 callers get queries and P as two fp16 parts each (22 bits) and twice
-// the products.  So that P fits fp16 whatever the value scales are, they are
-// divided by 2^k, k the exponent of the largest seen so far (O is rescaled
-// where it grows), and m follows the true maximum only where that is 7 binary
-// orders above it: P <= 2^7 2^8, and O is rescaled on few pages.
+//   e = 2^(f S - m),  l += e,  P = e,  O += P V
+// Every operand is brought into fp16's range by a power of two: a query row's
+// largest element to [2^10, 2^11) (16-bit queries stay exact), the keys of a
+// step to below 2^15 (f undoes both), the values to below 2^15 by that of the
+// largest scale so far (O is rescaled where it grows).  m follows the true
+// maximum only where that is 7 binary orders above it, so O is rescaled on few
+// steps.  What an operand rounds to:
+//   bf16  keys, values (code * scale) and P one fp16 each: 2^-11 a term, an
+//         eighth of the result's own rounding;
+//   fp16  keys in two parts (22 bits), values as bare codes (exact) with their
+//         scales on P, which rounds as the result does;
+//   fp32  as fp16, and queries and P in two parts: 2^-21 throughout.
+// The scales go into the operands because a scale a column costs the softmax
+// threads (thread = row) a shared-memory wavefront a column and warp: with both
+// scales there the pipe was as busy as the exponentials (967 us for 8192 rows
+// of 32 heads over 8).
 //
-// Warps: 4 softmax warps a tile (thread = row, so maximum and sum need no
-// exchange), 4 that convert pages (int8 in global memory -> fp16 tiles in
-// shared memory, 128-byte swizzled rows), 1 that issues every MMA.  P goes
-// back to TMEM, from where the second product takes it as its A operand.
+// Warps: 4 softmax warps a tile (maximum and sum need no exchange), 4 that
+// convert pages (int8 records -> fp16 tiles in shared memory, 128-byte
+// swizzled rows), 1 that copies the records, 1 a tile that issues its MMAs.  P goes back to TMEM, from where the
+// second product takes it as its A operand.
+//
+// A value scale that is no number would reach rows that do not see its
+// position through the product (0 * NaN): it is replaced by 0 and its key
+// scale by NaN, which only the rows that see the position take up.
+#include <float.h>
+
+#include <type_traits>
+
 #include "attention_math.cuh"
 #include "tc.cuh"
 
@@ -31,15 +45,33 @@ namespace {
 
 constexpr int kTileRows = 128;                 // MMA rows: TMEM lanes
 constexpr int kCtaRows = 2 * kTileRows;
-constexpr int kStages = 4;                     // converted pages in flight
-constexpr int kPromptThreads = 13 * 32;
-constexpr int kConvertWarp = 8, kMmaWarp = 12;
-constexpr int kTileBytes = kTileRows * kHeadDim * 2;   // 16 KB of queries
+constexpr int kConvertWarp = 8, kConvertWarps = 4, kMmaWarp = 12, kCopyWarp = 13;
+constexpr int kPromptThreads = 16 * 32;
+// Registers a thread: 128 at launch (512 threads); the softmax warps, which hold 128 scores a row, take over what the
+// converters and the last warpgroup (MMA and copies) give up: 2 * 184 + 96 + 48 = 4 * 128.
+constexpr int kSoftmaxRegs = 184, kConvertRegs = 96, kMmaRegs = 48;
+static_assert(2 * kSoftmaxRegs + kConvertRegs + kMmaRegs == 4 * 128, "the launch's registers, shared out");
+constexpr int kTileBytes = kTileRows * kHeadDim * 2;      // 16 KB of queries
 constexpr int kPageTile = kPagePositions * kHeadDim * 2;  // 8 KB of keys or values
 constexpr uint32_t kPromptWait = 1u << 22;     // waits of about a microsecond: a few seconds
-// TMEM columns: scores, outputs, probabilities (two fp16 a column) of both tiles
-constexpr int kColS = 0, kColO = 128, kColP = 256, kColLo = 64;
 constexpr int kTmemCols = 512;
+constexpr int kStagger = 4;                    // steps from which the tiles run half a step apart
+
+// The forms of the element types (above).  The second parts of fp32 leave
+// TMEM room for one page a step.
+template <class T>
+struct Step {
+    static constexpr bool kSplit = sizeof(T) == 4;                       // queries and P in two parts
+    static constexpr bool kFoldValues = __is_same(T, __nv_bfloat16);     // value scales on the values, else on P
+    static constexpr int kQParts = kSplit ? 2 : 1, kKParts = kFoldValues ? 1 : 2;
+    static constexpr int kPages = kSplit ? 1 : 2, kCols = kPages * kPagePositions;
+    static constexpr int kStages = kSplit ? 4 : 3;  // converted steps in flight
+    static constexpr int kRaw = 2;                  // steps of records as they lie in the pages
+    // TMEM columns: scores, outputs, probabilities (two fp16 a column; fp32: then their second parts) of both tiles
+    static constexpr int kS = 0, kO = 2 * kCols, kP = kO + 2 * kHeadDim, kPCols = kCols / 2;
+    static constexpr int kLo = 2 * kPCols;
+    static_assert(kP + 2 * kPCols * (kSplit ? 2 : 1) <= kTmemCols, "TMEM columns");
+};
 
 struct PromptArgs {
     const void *q;
@@ -51,13 +83,18 @@ struct PromptArgs {
     PagedCache c;
 };
 
-template <bool kSplit>
+template <class T>
 struct PromptSmem {
-    uint8_t q[2][kSplit ? 2 : 1][kTileBytes];  // 1024-byte aligned
-    uint8_t k[kStages][kPageTile], v[kStages][kPageTile];
-    float ks[kStages][kPagePositions], vs[kStages][kPagePositions];
-    int exponent[kStages];
-    uint64_t kv_full[kStages], kv_empty[kStages];
+    using St = Step<T>;
+    uint8_t q[2][St::kQParts][kTileBytes];  // 1024-byte aligned
+    uint8_t k[St::kStages][St::kKParts][St::kPages][kPageTile], v[St::kStages][St::kPages][kPageTile];
+    uint8_t raw[St::kRaw][St::kPages][kKvBlockBytes];
+    float scales[kConvertWarps][2][St::kPages][kPagePositions];  // each converter warp's copy: keys, values
+    float vs[St::kStages][St::kFoldValues ? 4 : St::kCols];
+    float key_factor[St::kStages];  // 2^(the keys' exponent), the scale of their scores
+    int exponent[St::kStages];      // of the value scales so far
+    uint64_t raw_full[St::kRaw], kv_full[St::kStages], kv_empty[St::kStages];
+    int missing[St::kRaw];  // bit g: the step's page g is not in the pool
     uint64_t s_full[2], s_free[2], p_full[2], pv_done[2];
     uint32_t tmem;
     int seq, tile;  // this CTA's work: sequence (-1: none) and 256-row tile of it
@@ -68,36 +105,43 @@ struct PromptSmem {
 constexpr uint32_t idesc_f16(int m, int n) {
     return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
+// Warp-converged: every lane calls, one elected lane issues.
 __device__ __forceinline__ void mma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
     asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+        "{\n .reg .pred p, e;\n elect.sync _|e, 0xffffffff;\n setp.ne.b32 p, %4, 0;\n"
+        " @e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
         "l"(a), "l"(b), "r"(idesc), "r"(acc)
         : "memory");
 }
 __device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
     asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+        "{\n .reg .pred p, e;\n elect.sync _|e, 0xffffffff;\n setp.ne.b32 p, %4, 0;\n"
+        " @e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
         "r"(a), "l"(b), "r"(idesc), "r"(acc)
         : "memory");
 }
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
     asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,"
-        "%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::"r"(r[0]),
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(
+            r[0]),
         "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
-        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]),
-        "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
-        "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
-        : "memory");
+        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr));
+}
+// Bounded wait of a whole warp: a plain test first (the phase is mostly complete already), then suspending ones.
+__device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity, volatile int *abort) {
+    if (__all_sync(0xffffffffu, mbar_test_wait(bar, parity))) return true;
+    const bool ok = mbar_wait_bounded(bar, parity, kPromptWait);
+    return __all_sync(0xffffffffu, ok && !*abort);
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-template <class T, bool kSplit>
+template <class T>
 __global__ void __launch_bounds__(kPromptThreads, 1) attention_prompt_kernel(PromptArgs a) {
+    using St = Step<T>;
+    constexpr bool kSplit = St::kSplit;
+    constexpr int kStages = St::kStages, kPages = St::kPages, kCols = St::kCols;
     extern __shared__ uint8_t smem_raw[];
-    PromptSmem<kSplit> &s = *reinterpret_cast<PromptSmem<kSplit> *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
-                                                                     ~uintptr_t(1023));
+    PromptSmem<T> &s =
+        *reinterpret_cast<PromptSmem<T> *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int kv_head = blockIdx.x % a.c.heads, work = blockIdx.x / a.c.heads;
     const int group = a.heads / a.c.heads;
@@ -136,7 +180,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attention_prompt_kernel(Pro
             }
     } else if (warp == kMmaWarp) {
         if (lane == 0) {
-            for (int i = 0; i < kStages; i++) mbar_init(&s.kv_full[i], 4), mbar_init(&s.kv_empty[i], 1);
+            for (int i = 0; i < St::kRaw; i++) mbar_init(&s.raw_full[i], 1);
+            for (int i = 0; i < kStages; i++) mbar_init(&s.kv_full[i], kConvertWarps), mbar_init(&s.kv_empty[i], 2);
             for (int t = 0; t < 2; t++)
                 mbar_init(&s.s_full[t], 1), mbar_init(&s.s_free[t], 4), mbar_init(&s.p_full[t], 4),
                     mbar_init(&s.pv_done[t], 1);
@@ -157,23 +202,26 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attention_prompt_kernel(Pro
     const bool ok_seq = slot >= 0 && slot < a.c.slots && start >= 0 &&
                         (long long)start + n <= (long long)a.c.max_pages * kPagePositions;
     const long long packed = (long long)n * group, m0 = (long long)s.tile * kCtaRows;
-    // pages [lo, hi] of each tile (hi < lo: no rows)
-    int lo[2], hi[2];
+    // the pages its rows see, from page0 on in steps; steps [lo, hi] of each tile (hi < lo: no rows)
+    int lo[2], hi[2], page0 = 0;
 #pragma unroll
     for (int t = 0; t < 2; t++) {
         const long long b = m0 + t * kTileRows, e = min(packed, b + kTileRows);
         lo[t] = 0, hi[t] = -1;
         if (seq >= 0 && ok_seq && b < e) {
             const int from = start + (int)(b / group), to = start + (int)((e - 1) / group);
-            lo[t] = a.window ? max(0, from - a.window + 1) / kPagePositions : 0;
-            hi[t] = to / kPagePositions;
+            const int first = a.window ? max(0, from - a.window + 1) / kPagePositions : 0;
+            if (t == 0) page0 = first;
+            lo[t] = (first - page0) / kPages;
+            hi[t] = (to / kPagePositions - page0) / kPages;
         }
     }
-    const int page0 = lo[0], page1 = max(hi[0], hi[1]);
+    const int steps = max(hi[0], hi[1]) + 1;
     const int last_pos = start + (int)((min(packed, m0 + kCtaRows) - 1) / group);  // the CTA's last query
 
     if (warp < kConvertWarp) {
         // ------------------------------------------------------- softmax --
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
         const int t = warp >> 2, row = threadIdx.x & (kTileRows - 1);
         const long long m = m0 + t * kTileRows + row;
         const bool valid = seq >= 0 && m < packed;
@@ -213,101 +261,102 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attention_prompt_kernel(Pro
         fence_proxy_async_smem();
         __syncthreads();
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-        const uint32_t ts = tmem + lanes + kColS + t * 64, to = tmem + lanes + kColO + t * 64;
-        const uint32_t tp = tmem + lanes + kColP + t * 32;
+        const uint32_t ts = tmem + lanes + St::kS + t * kCols, to = tmem + lanes + St::kO + t * kHeadDim;
+        const uint32_t tp = tmem + lanes + St::kP + t * St::kPCols;
         float top = -INFINITY, total = 0.0f;
         int exponent = kMinExponent;
         bool ok = true;
         for (int i = lo[t]; i <= hi[t]; i++) {
-            const int it = i - lo[t], st = (i - page0) % kStages;
-            ok = mbar_wait_bounded(&s.s_full[t], it & 1, kPromptWait) &&
-                 mbar_wait_bounded(&s.kv_full[st], ((i - page0) / kStages) & 1, kPromptWait);
-            if (!__all_sync(0xffffffffu, ok) || s.abort) break;
+            const int it = i - lo[t], st = i % kStages;
+            ok = warp_wait(&s.s_full[t], it & 1, &s.abort) && warp_wait(&s.kv_full[st], (i / kStages) & 1, &s.abort);
+            if (!ok) break;
             tc_fence_after();
-            uint32_t r0[32], r1[32];
-            tmem_ld32(ts, r0);
-            tmem_ld32(ts + 32, r1);
-            tmem_ld_wait(r0);
-            tmem_ld_wait(r1);
+            uint32_t r[kCols];
+#pragma unroll
+            for (int c = 0; c < kCols; c += 32) tmem_ld32(ts + c, reinterpret_cast<uint32_t(&)[32]>(r[c]));
+            tmem_ld_wait(r);
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&s.s_free[t]);
-            float x[64];
-            const float4 *ks = reinterpret_cast<const float4 *>(s.ks[st]);
-#pragma unroll
-            for (int j = 0; j < 64; j += 4) {
-                const float4 c = ks[j >> 2];
-                const uint32_t *r = j < 32 ? r0 + j : r1 + (j - 32);
-                x[j] = __uint_as_float(r[0]) * c.x, x[j + 1] = __uint_as_float(r[1]) * c.y;
-                x[j + 2] = __uint_as_float(r[2]) * c.z, x[j + 3] = __uint_as_float(r[3]) * c.w;
-            }
-            // positions this row does not see
-            const int upto = pos - i * kPagePositions;
+            // positions [from, upto] of the step are this row's
+            const int upto = pos - (page0 + i * kPages) * kPagePositions;
             const int from = a.window ? upto - a.window + 1 : 0;
-            const bool whole = __all_sync(0xffffffffu, upto >= kPagePositions - 1 && from <= 0);
-            if (!whole) {
-#pragma unroll
-                for (int j = 0; j < 64; j++)
-                    if (j > upto || j < from) x[j] = -INFINITY;
-            }
-            float peak = x[0];
-#pragma unroll
-            for (int j = 1; j < 64; j++) peak = fmaxf(peak, x[j]);
+            const bool whole = __all_sync(0xffffffffu, upto >= kCols - 1 && from <= 0);
             const int ke = s.exponent[st];
-            float keep = 1.0f;
-            const bool grew = (peak - top) * scale_q > kLazy || (top == -INFINITY && peak > -INFINITY);
-            if (grew) {
-                keep = exp2_approx((top - peak) * scale_q);
-                if (top == -INFINITY) keep = 0.0f;
-                total *= keep;
-                top = peak;
-            }
-            if (ke > exponent) keep *= exp2_approx((float)(exponent - ke));
-            exponent = ke;
-            const float base = top == -INFINITY ? 0.0f : top * scale_q;
-            uint32_t hp[32], lp[kSplit ? 32 : 1];
-            const float4 *vs = reinterpret_cast<const float4 *>(s.vs[st]);
-            float sum0 = 0.0f, sum1 = 0.0f;
+            const float f = fminf(fmaxf(scale_q * s.key_factor[st], FLT_MIN), FLT_MAX);  // it multiplies infinities
+            // two copies, so that steps every row sees whole carry no masks
+            const auto step = [&](auto masked) {
+                if constexpr (decltype(masked)::value) {
 #pragma unroll
-            for (int j = 0; j < 64; j += 4) {
-                const float4 c = vs[j >> 2];
-                float e[4], p[4];
-#pragma unroll
-                for (int u = 0; u < 4; u++) e[u] = exp2_approx(fmaf(x[j + u], scale_q, -base));
-                sum0 += e[0] + e[2], sum1 += e[1] + e[3];
-                p[0] = e[0] * c.x, p[1] = e[1] * c.y, p[2] = e[2] * c.z, p[3] = e[3] * c.w;
-                if (!whole) {
-#pragma unroll
-                    for (int u = 0; u < 4; u++)
-                        if (j + u > upto || j + u < from) p[u] = 0.0f;
+                    for (int j = 0; j < kCols; j++)
+                        if (j > upto || j < from) r[j] = __float_as_uint(-INFINITY);
                 }
-                hp[j >> 1] = half_pair(p[0], p[1]), hp[(j >> 1) + 1] = half_pair(p[2], p[3]);
-                if constexpr (kSplit)
-                    lp[kSplit ? j >> 1 : 0] = half_rest(p[0], p[1], hp[j >> 1]),
-                    lp[kSplit ? (j >> 1) + 1 : 0] = half_rest(p[2], p[3], hp[(j >> 1) + 1]);
-            }
-            total += sum0 + sum1;
-            // the previous product has read P and finished O
-            if (it > 0) {
-                ok = mbar_wait_bounded(&s.pv_done[t], (it - 1) & 1, kPromptWait);
-                if (!__all_sync(0xffffffffu, ok)) break;
-                tc_fence_after();
-                if (__any_sync(0xffffffffu, keep != 1.0f)) {
-                    tmem_ld32(to, r0);
-                    tmem_ld32(to + 32, r1);
-                    tmem_ld_wait(r0);
-                    tmem_ld_wait(r1);
+                float peaks[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                    for (int j = 0; j < 32; j++) {
-                        r0[j] = __float_as_uint(__uint_as_float(r0[j]) * keep);
-                        r1[j] = __float_as_uint(__uint_as_float(r1[j]) * keep);
+                for (int j = 0; j < kCols; j += 2)
+                    peaks[(j >> 1) & 3] = fmaxf(peaks[(j >> 1) & 3], fmaxf(__uint_as_float(r[j]), __uint_as_float(r[j + 1])));
+                const float peak = fmaxf(fmaxf(peaks[0], peaks[1]), fmaxf(peaks[2], peaks[3])) * f;
+                float keep = 1.0f;
+                if (peak - top > kLazy || (top == -INFINITY && peak > -INFINITY)) {
+                    keep = top == -INFINITY ? 0.0f : exp2_approx(top - peak);
+                    total *= keep;
+                    top = peak;
+                }
+                if (ke > exponent) keep *= exp2_approx((float)(exponent - ke));
+                exponent = ke;
+                // the previous product has read P and finished O
+                if (it > 0) {
+                    ok = warp_wait(&s.pv_done[t], (it - 1) & 1, &s.abort);
+                    if (!ok) return;
+                    tc_fence_after();
+                    if (__any_sync(0xffffffffu, keep != 1.0f)) {
+#pragma unroll
+                        for (int c = 0; c < kHeadDim; c += 16) {
+                            uint32_t o[16];
+                            tmem_ld16(to + c, o);
+                            tmem_ld_wait(o);
+#pragma unroll
+                            for (int j = 0; j < 16; j++) o[j] = __float_as_uint(__uint_as_float(o[j]) * keep);
+                            tmem_st16(to + c, o);
+                        }
                     }
-                    tmem_st32(to, r0);
-                    tmem_st32(to + 32, r1);
                 }
-            }
-            tmem_st32(tp, hp);
-            if constexpr (kSplit) tmem_st32(tp + kColLo, reinterpret_cast<const uint32_t(&)[32]>(lp));
+                // folded value scales leave P room up to 2^15
+                const float base = (top == -INFINITY ? 0.0f : top) - (St::kFoldValues ? 8.0f : 0.0f);
+                [[maybe_unused]] const ulonglong2 *vs = reinterpret_cast<const ulonglong2 *>(s.vs[st]);
+                const uint64_t f2 = f2_pack(f, f), base2 = f2_pack(-base, -base);
+                uint64_t sums[2] = {0, 0};
+#pragma unroll
+                for (int c = 0; c < kCols; c += 32) {
+                    uint32_t hp[16];
+                    [[maybe_unused]] uint32_t lp[kSplit ? 16 : 1];
+#pragma unroll
+                    for (int j = 0; j < 32; j += 4) {
+                        [[maybe_unused]] ulonglong2 v2;
+                        if constexpr (!St::kFoldValues) v2 = vs[(c + j) / 4];
+#pragma unroll
+                        for (int u = 0; u < 2; u++) {
+                            const int k = c + j + 2 * u;
+                            float e0, e1;
+                            f2_unpack(f2_fma(f2_pack(__uint_as_float(r[k]), __uint_as_float(r[k + 1])), f2, base2), e0, e1);
+                            e0 = exp2_approx(e0), e1 = exp2_approx(e1);
+                            const uint64_t e = f2_pack(e0, e1);
+                            sums[u] = f2_add(sums[u], e);
+                            if constexpr (!St::kFoldValues) f2_unpack(f2_mul(e, u ? v2.y : v2.x), e0, e1);
+                            hp[j / 2 + u] = half_pair(e0, e1);
+                            if constexpr (kSplit) lp[kSplit ? j / 2 + u : 0] = half_rest(e0, e1, hp[j / 2 + u]);
+                        }
+                    }
+                    tmem_st16(tp + c / 2, hp);
+                    if constexpr (kSplit) tmem_st16(tp + St::kLo + c / 2, reinterpret_cast<const uint32_t(&)[16]>(lp));
+                }
+                float sum0, sum1;
+                f2_unpack(f2_add(sums[0], sums[1]), sum0, sum1);
+                total += sum0 + sum1;
+            };
+            if (whole) step(std::false_type{});
+            else step(std::true_type{});
+            if (!ok) break;
             tmem_st_wait();
             tc_fence_before();
             __syncwarp();
@@ -315,8 +364,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attention_prompt_kernel(Pro
         }
         // the rows' results
         if (hi[t] >= lo[t]) {
-            ok = ok && !s.abort && mbar_wait_bounded(&s.pv_done[t], (hi[t] - lo[t]) & 1, kPromptWait);
-            ok = __all_sync(0xffffffffu, ok);
+            ok = ok && warp_wait(&s.pv_done[t], (hi[t] - lo[t]) & 1, &s.abort);
             if (!ok) {
                 s.abort = 1;
                 if (lane == 0 && a.c.status) atomicOr(a.c.status, kStatusTimeout);
@@ -350,150 +398,213 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attention_prompt_kernel(Pro
         }
     } else if (warp < kMmaWarp) {
         // -------------------------------------------------- page converter --
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kConvertRegs));
         const int c = warp - kConvertWarp;
         int exponent = kMinExponent;
-        int ids = 0;
-        struct Page {
-            uint4 k[2], v[2];
-            float2 scale;
-            int id;
-        } cur, nxt;
         const float fold = a.scale * kLog2E;
-        auto fetch = [&](int i, Page &p) {
-            const int rel = i - page0;
-            if ((rel & 31) == 0) ids = i + lane <= page1 ? cache_page(a.c, slot, i + lane) : -1;
-            p.id = __shfl_sync(0xffffffffu, ids, rel & 31);
-            if (p.id < 0) return;
-            const uint8_t *rec = cache_record(a.c, p.id, kv_head);
-#pragma unroll
-            for (int u = 0; u < 2; u++) {
-                // keys: lane -> (row & 7 = lane & 7, 4-dim column lane >> 3) of a 512-byte block; values: dim and 16
-                // positions
-                p.k[u] = __ldg(reinterpret_cast<const uint4 *>(rec + (c * 2 + u) * 512 + ((lane & 7) * 4 + (lane >> 3)) * 16));
-                const int d = (c * 2 + u) * 8 + (lane & 7);
-                p.v[u] = __ldg(reinterpret_cast<const uint4 *>(rec + kVOffset + d * 64 + (((lane >> 3) ^ ((d >> 1) & 3)) << 4)));
-            }
-            if (c == 0) {  // key scales of positions lane, lane + 32
-                p.scale.x = __ldg(reinterpret_cast<const float *>(rec + kKScaleOffset) + k_scale_index(lane));
-                p.scale.y = __ldg(reinterpret_cast<const float *>(rec + kKScaleOffset) + k_scale_index(lane + 32));
-            } else if (c == 1) {
-                p.scale.x = __ldg(reinterpret_cast<const float *>(rec + kVScaleOffset) + lane);
-                p.scale.y = __ldg(reinterpret_cast<const float *>(rec + kVScaleOffset) + lane + 32);
-            }
-        };
-        if (page0 <= page1) fetch(page0, cur);
         __syncthreads();
-        for (int i = page0; i <= page1; i++) {
-            if (i < page1) fetch(i + 1, nxt);
-            const int rel = i - page0, st = rel % kStages;
-            if (rel >= kStages) {
-                const bool ok = mbar_wait_bounded(&s.kv_empty[st], ((rel / kStages) - 1) & 1, kPromptWait);
-                if (!__all_sync(0xffffffffu, ok) || s.abort) {
-                    s.abort = 1;
-                    if (lane == 0 && !ok && a.c.status) atomicOr(a.c.status, kStatusTimeout);
-                    break;
+        for (int i = 0; i < steps; i++) {
+            const int st = i % kStages, rs = i % St::kRaw;
+            if (!warp_wait(&s.raw_full[rs], (i / St::kRaw) & 1, &s.abort) ||
+                (i >= kStages && !warp_wait(&s.kv_empty[st], ((i / kStages) - 1) & 1, &s.abort))) {
+                if (lane == 0 && !s.abort && a.c.status) atomicOr(a.c.status, kStatusTimeout);
+                s.abort = 1;
+                break;
+            }
+            // The scales, lane -> positions lane and lane + 32: those behind the CTA's last query belong to no one, the
+            // keys' of a missing page are NaN, and those of a position whose value scale is no number.
+            const int missing = s.missing[rs];
+            float ks[kPages][2], vs[kPages][2];
+            int key_top = 0, value_top = 0;
+#pragma unroll
+            for (int g = 0; g < kPages; g++) {
+                const int seen = last_pos - (page0 + i * kPages + g) * kPagePositions;
+                const uint8_t *rec = s.raw[rs][g];
+                if ((missing >> g & 1) && c == 0 && lane == 0 && a.c.status) atomicOr(a.c.status, kStatusBadPage);
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const int p = lane + 32 * h;
+                    float k = reinterpret_cast<const float *>(rec + kKScaleOffset)[k_scale_index(p)] * fold;
+                    float v = reinterpret_cast<const float *>(rec + kVScaleOffset)[v_scale_index(p)];
+                    if ((missing >> g & 1) || !(fabsf(v) <= FLT_MAX)) k = __int_as_float(0x7fc00000), v = 0.0f;
+                    if (p > seen) k = 0.0f, v = 0.0f;
+                    ks[g][h] = k, vs[g][h] = v;
+                    key_top = max(key_top, scale_exponent(k)), value_top = max(value_top, scale_exponent(v));
                 }
             }
-            const bool there = cur.id >= 0;
-            if (!there) {
+            const int key_exponent = max(kMinExponent, __reduce_max_sync(0xffffffffu, key_top) - 126);
+            exponent = max(exponent, __reduce_max_sync(0xffffffffu, value_top) - 126);
+            const float key_norm = pow2(8 - key_exponent), value_norm = pow2(8 - exponent);  // exponents in [-110, 128]
+            if (c == 0 && lane == 0) s.key_factor[st] = pow2(key_exponent - 8), s.exponent[st] = exponent;
 #pragma unroll
-                for (int u = 0; u < 2; u++) cur.k[u] = cur.v[u] = make_uint4(0, 0, 0, 0);
-                if (lane == 0 && c == 0 && a.c.status) atomicOr(a.c.status, kStatusBadPage);
-            }
+            for (int g = 0; g < kPages; g++)
 #pragma unroll
-            for (int u = 0; u < 2; u++) {
-                const int block = c * 2 + u;  // (16-row tile, 32-dim step)
-                const int row = (block >> 1) * 16 + (lane & 7), j = (block & 1) * 4 + (lane >> 3);
-                uint4 a0, a1;
-                codes_to_half(cur.k[u].x, a0.x, a0.y);
-                codes_to_half(cur.k[u].z, a0.z, a0.w);
-                codes_to_half(cur.k[u].y, a1.x, a1.y);
-                codes_to_half(cur.k[u].w, a1.z, a1.w);
-                const int byte = row * 128 + ((j ^ (row & 7)) << 4);
-                *reinterpret_cast<uint4 *>(&s.k[st][byte]) = a0;
-                *reinterpret_cast<uint4 *>(&s.k[st][byte + 8 * 128]) = a1;
-                const int d = block * 8 + (lane & 7), jv = (lane >> 3) * 2;
-                codes_to_half(cur.v[u].x, a0.x, a0.y);
-                codes_to_half(cur.v[u].y, a0.z, a0.w);
-                codes_to_half(cur.v[u].z, a1.x, a1.y);
-                codes_to_half(cur.v[u].w, a1.z, a1.w);
-                *reinterpret_cast<uint4 *>(&s.v[st][d * 128 + ((jv ^ (d & 7)) << 4)]) = a0;
-                *reinterpret_cast<uint4 *>(&s.v[st][d * 128 + (((jv + 1) ^ (d & 7)) << 4)]) = a1;
-            }
-            // scales; those behind the CTA's last query belong to no one
-            const int seen = last_pos - i * kPagePositions;
-            float2 f = cur.scale;
-            if (!there) f.x = f.y = __int_as_float(0x7fc00000);
-            if (lane > seen) f.x = 0.0f;
-            if (lane + 32 > seen) f.y = 0.0f;
-            if (c == 0) {
-                s.ks[st][lane] = f.x * fold;
-                s.ks[st][lane + 32] = f.y * fold;
-            } else if (c == 1) {
-                if (!there) f.x = f.y = 0.0f;
-                const int e = __reduce_max_sync(0xffffffffu, max(scale_exponent(f.x), scale_exponent(f.y)));
-                exponent = max(exponent, e - 126);
-                const float down = pow2(8 - exponent);  // -110 <= exponent <= 128
-                s.vs[st][lane] = f.x * down;
-                s.vs[st][lane + 32] = f.y * down;
-                if (lane == 0) s.exponent[st] = exponent;
+                for (int h = 0; h < 2; h++) {
+                    const int p = lane + 32 * h;
+                    const float k = ks[g][h] * key_norm, v = vs[g][h] * value_norm;
+                    if constexpr (St::kFoldValues) {  // the key scale as two fp16, the value scale as one
+                        const uint32_t kh = half_pair(k, 0.0f);
+                        reinterpret_cast<uint32_t *>(s.scales[c][0][g])[p] = half_pair(k, k - __low2float(as_half2(kh)));
+                        reinterpret_cast<__half *>(s.scales[c][1][g])[p] = __float2half_rn(v);
+                    } else {
+                        s.scales[c][0][g][p] = k;
+                        if (c == 0) s.vs[st][g * kPagePositions + p] = v;
+                    }
+                }
+            __syncwarp();
+            // A warp takes 16 positions of a page's keys and 16 dims of its values: two 512-byte blocks of each.
+            uint4 kw[kPages][2], vw[kPages][2];
+#pragma unroll
+            for (int g = 0; g < kPages; g++)
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    // keys: lane -> row lane & 7 (and + 8), 4-dim column lane >> 3 of dims 32 u ..; values: lane -> dim
+                    // lane & 7, positions 16 (lane >> 3) ..
+                    const uint8_t *rec = s.raw[rs][g];
+                    kw[g][u] = *reinterpret_cast<const uint4 *>(rec + (2 * c + u) * 512 + ((lane & 7) * 4 + (lane >> 3)) * 16);
+                    const int d = (2 * c + u) * 8 + (lane & 7);
+                    vw[g][u] = *reinterpret_cast<const uint4 *>(rec + kVOffset + d * 64 + (((lane >> 3) ^ ((d >> 1) & 3)) << 4));
+                }
+#pragma unroll
+            for (int g = 0; g < kPages; g++) {
+                const int row = c * 16 + (lane & 7);
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const float sc = s.scales[c][0][g][row + 8 * h];
+                    const uint32_t sh = __byte_perm(__float_as_uint(sc), 0, 0x1010), sl = __byte_perm(__float_as_uint(sc), 0, 0x3232);
+#pragma unroll
+                    for (int u = 0; u < 2; u++) {
+                        // words: (row, dims), (row + 8, dims), then dims + 16
+                        const uint32_t w0 = h ? kw[g][u].y : kw[g][u].x, w1 = h ? kw[g][u].w : kw[g][u].z;
+                        const int at = (row + 8 * h) * 128 + (((u * 4 + (lane >> 3)) ^ (row & 7)) << 4);
+                        uint32_t hi[4], lo[4];
+                        if constexpr (St::kFoldValues) {
+                            folded_codes(w0, sh, sl, hi[0], hi[1]);
+                            folded_codes(w1, sh, sl, hi[2], hi[3]);
+                        } else {
+                            scaled_codes(w0, sc, hi[0], hi[1], lo[0], lo[1]);
+                            scaled_codes(w1, sc, hi[2], hi[3], lo[2], lo[3]);
+                            *reinterpret_cast<uint4 *>(&s.k[st][St::kKParts - 1][g][at]) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                        }
+                        *reinterpret_cast<uint4 *>(&s.k[st][0][g][at]) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                    }
+                }
+                uint32_t f[8];
+                if constexpr (St::kFoldValues) {
+                    const uint4 *sc = reinterpret_cast<const uint4 *>(s.scales[c][1][g]) + (lane >> 3) * 2;
+                    const uint4 s0 = sc[0], s1 = sc[1];
+                    f[0] = s0.x, f[1] = s0.y, f[2] = s0.z, f[3] = s0.w, f[4] = s1.x, f[5] = s1.y, f[6] = s1.z, f[7] = s1.w;
+                }
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    const uint32_t words[4] = {vw[g][u].x, vw[g][u].y, vw[g][u].z, vw[g][u].w};
+                    uint32_t h[8];
+#pragma unroll
+                    for (int j = 0; j < 4; j++) codes_to_half(words[j], h[2 * j], h[2 * j + 1]);
+                    if constexpr (St::kFoldValues) {
+#pragma unroll
+                        for (int j = 0; j < 8; j++) h[j] = half2_bits(__hmul2(as_half2(h[j]), as_half2(f[j])));
+                    }
+                    const int d = (2 * c + u) * 8 + (lane & 7), j = (lane >> 3) * 2;
+                    *reinterpret_cast<uint4 *>(&s.v[st][g][d * 128 + ((j ^ (d & 7)) << 4)]) = make_uint4(h[0], h[1], h[2], h[3]);
+                    *reinterpret_cast<uint4 *>(&s.v[st][g][d * 128 + (((j + 1) ^ (d & 7)) << 4)]) =
+                        make_uint4(h[4], h[5], h[6], h[7]);
+                }
             }
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(&s.kv_full[st]);
-            cur = nxt;
         }
     } else {
         // ------------------------------------------------------ MMA issuer --
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kMmaRegs));
         __syncthreads();
-        if (lane == 0 && page0 <= page1) {
-            const uint32_t idesc = idesc_f16(kTileRows, kPagePositions);
-            bool ok = true;
-            auto scores = [&](int t, int i) {
-                if (!ok || i < lo[t] || i > hi[t]) return;
-                const int it = i - lo[t], rel = i - page0, st = rel % kStages;
-                ok = mbar_wait_bounded(&s.kv_full[st], (rel / kStages) & 1, kPromptWait) &&
-                     (it == 0 || mbar_wait_bounded(&s.s_free[t], (it - 1) & 1, kPromptWait));
-                if (!ok) return;
-                tc_fence_after();
-                const uint64_t b = sw128_kmajor_desc(s.k[st]);
+        bool ok = true;
+        if (warp == kCopyWarp) {
+            // the records of each step into their ring, once the converters have read the step kRaw before
+            const int page_end = last_pos / kPagePositions + 1;
+            int ids = -1, i = 0;
+            for (; i < steps; i++) {
+                const int rs = i % St::kRaw;
+                int absent = 0, found = 0, id[kPages];
 #pragma unroll
-                for (int part = 0; part < (kSplit ? 2 : 1); part++) {
-                    const uint64_t q = sw128_kmajor_desc(s.q[t][part]);
-#pragma unroll
-                    for (int k = 0; k < 4; k++)
-                        mma_f16_ss(tmem + kColS + t * 64, q + 2 * k, b + 2 * k, idesc, part + k > 0);
+                for (int g = 0; g < kPages; g++) {
+                    const int rel = i * kPages + g, page = page0 + rel;
+                    if ((rel & 31) == 0) ids = page + lane < page_end ? cache_page(a.c, slot, page + lane) : -1;
+                    id[g] = __shfl_sync(0xffffffffu, ids, rel & 31);
+                    if (id[g] >= 0) found++;
+                    else if (page < page_end) absent |= 1 << g;  // behind the last page there is nothing to miss
                 }
-                mma_commit(&s.s_full[t]);
-            };
-            auto values = [&](int t, int i) {
+                if (i >= St::kRaw) {
+                    const int j = i - St::kRaw;
+                    ok = warp_wait(&s.kv_full[j % kStages], (j / kStages) & 1, &s.abort);
+                    if (!ok) break;
+                }
+                if (lane == 0) {
+                    s.missing[rs] = absent;
+                    if (found) mbar_arrive_expect_tx(&s.raw_full[rs], found * kKvBlockBytes);
+                    else mbar_arrive(&s.raw_full[rs]);
+#pragma unroll
+                    for (int g = 0; g < kPages; g++)
+                        if (id[g] >= 0)
+                            bulk_g2s(s.raw[rs][g], cache_record(a.c, id[g], kv_head), kKvBlockBytes, &s.raw_full[rs]);
+                }
+                __syncwarp();
+            }
+            // every copy in flight lands before the CTA exits (bounded)
+            if (!ok)
+                for (int j = max(0, i - St::kRaw); j < i; j++)
+                    mbar_wait_bounded(&s.raw_full[j % St::kRaw], (j / St::kRaw) & 1, kPromptWait);
+        } else if (warp == kMmaWarp || warp == kMmaWarp + 2) {
+            // A warp issues the products of one tile.
+            constexpr uint32_t idesc_s = idesc_f16(kTileRows, kCols), idesc_o = idesc_f16(kTileRows, kHeadDim);
+            const int t = (warp - kMmaWarp) >> 1;
+            const uint32_t ts = tmem + St::kS + t * kCols, to = tmem + St::kO + t * kHeadDim, tp = tmem + St::kP + t * St::kPCols;
+            auto scores = [&](int i) {
                 if (!ok || i < lo[t] || i > hi[t]) return;
-                const int it = i - lo[t], st = (i - page0) % kStages;
-                ok = mbar_wait_bounded(&s.p_full[t], it & 1, kPromptWait);
+                const int it = i - lo[t], st = i % kStages;
+                ok = warp_wait(&s.kv_full[st], (i / kStages) & 1, &s.abort) &&
+                     (it == 0 || warp_wait(&s.s_free[t], (it - 1) & 1, &s.abort));
                 if (!ok) return;
                 tc_fence_after();
-                const uint64_t b = sw128_kmajor_desc(s.v[st]);
 #pragma unroll
-                for (int part = 0; part < (kSplit ? 2 : 1); part++)
+                for (int qp = 0; qp < St::kQParts; qp++)
 #pragma unroll
-                    for (int k = 0; k < 4; k++)
-                        mma_f16_ts(tmem + kColO + t * 64, tmem + kColP + t * 32 + part * kColLo + k * 8, b + 2 * k,
-                                   idesc, it + part + k > 0);
-                mma_commit(&s.pv_done[t]);
+                    for (int kp = 0; kp < St::kKParts - (qp ? 1 : 0); kp++) {  // not the second parts of both
+                        const uint64_t q = sw128_kmajor_desc(s.q[t][qp]), b = sw128_kmajor_desc(s.k[st][kp]);
+#pragma unroll
+                        for (int k = 0; k < 4; k++) mma_f16_ss(ts, q + 2 * k, b + 2 * k, idesc_s, qp + kp + k > 0);
+                    }
+                mma_commit_elect(&s.s_full[t]);
             };
-            scores(0, page0);
-            scores(1, page0);
-            for (int i = page0; i <= page1 && ok && !s.abort; i++) {
-                scores(0, i + 1);
-                scores(1, i + 1);
-                values(0, i);
-                values(1, i);
-                if (ok) mma_commit(&s.kv_empty[(i - page0) % kStages]);
+            // The tiles run half a step apart, so that one's maxima and waits pass under the other's exponentials: tile
+            // 1 begins when tile 0 has its first probabilities.
+            if (t == 1 && steps >= kStagger) ok = warp_wait(&s.p_full[0], 0, &s.abort);
+            scores(0);
+            for (int i = 0; i < steps && ok; i++) {
+                scores(i + 1);
+                const int it = i - lo[t], st = i % kStages;
+                if (i >= lo[t] && i <= hi[t]) {
+                    ok = ok && warp_wait(&s.p_full[t], it & 1, &s.abort);
+                    if (!ok) break;
+                    tc_fence_after();
+#pragma unroll
+                    for (int part = 0; part < (kSplit ? 2 : 1); part++)
+#pragma unroll
+                        for (int k = 0; k < 4 * kPages; k++)
+                            mma_f16_ts(to, tp + part * St::kLo + k * 8, sw128_kmajor_desc(s.v[st][k >> 2]) + 2 * (k & 3), idesc_o,
+                                       it + part + k > 0);
+                    mma_commit_elect(&s.pv_done[t]);
+                } else {  // the step is the other tile's alone
+                    ok = warp_wait(&s.kv_full[st], (i / kStages) & 1, &s.abort);
+                    if (!ok) break;
+                }
+                mma_commit_elect(&s.kv_empty[st]);
             }
-            if (!ok) {
-                s.abort = 1;
-                if (a.c.status) atomicOr(a.c.status, kStatusTimeout);
-            }
+        }
+        if (!ok) {
+            s.abort = 1;
+            if (lane == 0 && a.c.status) atomicOr(a.c.status, kStatusTimeout);
         }
         __syncwarp();
     }
@@ -532,9 +643,8 @@ extern "C" NDL_API int ndl_attention_prompt(const void *q, long long q_stride, i
                 sequences);
     return with_type(type, [&](auto t) {
         using T = decltype(t);
-        constexpr bool kSplit = sizeof(T) == 4;
-        const auto kernel = attention_prompt_kernel<T, kSplit>;
-        constexpr size_t smem = sizeof(PromptSmem<kSplit>) + 1024;
+        const auto kernel = attention_prompt_kernel<T>;
+        constexpr size_t smem = sizeof(PromptSmem<T>) + 1024;
         static DeviceOnce attribute;  // the attribute belongs to the kernel on one device
         const int st = attribute.run([&] {
             const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);

@@ -174,61 +174,76 @@ def attention_paged(q8, qs, row_slot, row_pos, page_table, pool, page_bytes, lay
 
 # ------------------------------- rows, attention and logits over own pages --
 
+# A call's checks read each tensor attribute once: they are most of a small call's time on the host.
+
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+_I32, _F32, _U8 = torch.int32, torch.float32, torch.uint8
 
 
-def _type(t, name):
-    if not isinstance(t, torch.Tensor) or t.dtype not in _TYPES:
-        raise TypeError(f"{name} must be a float32, float16 or bfloat16 tensor")
-    return _TYPES[t.dtype]
+def _start(t, name, types=_TYPES):
+    """(element type code, device index) of the operand that decides a call's type and device."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise TypeError(f"{name} must be a CUDA tensor")
+    code = types.get(t.dtype)
+    if code is None:
+        raise TypeError(f"{name} must be one of {list(types)}, got {t.dtype}")
+    return code, t.get_device()
 
 
-def _heads(t, dtype, name, device, shape=None):
-    """Address and row stride of a [rows, heads, 64] operand whose rows may be strided (a projection's columns)."""
+def _wrong(t, dtype, name, index, numel=None):
+    """What keeps an operand from being a contiguous `dtype` tensor of `numel` elements on the device."""
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise TypeError(f"{name} must be a CUDA tensor")
     if t.dtype != dtype:
         raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
-    if t.device != device:
-        raise ValueError(f"{name} is on {t.device}, not on {device}")
-    if t.dim() != 3 or t.shape[2] != 64 or (shape is not None and tuple(t.shape) != tuple(shape)):
+    if t.get_device() != index:
+        raise ValueError(f"{name} is on {t.device}, not on cuda:{index}")
+    if numel is not None and t.numel() != numel:
+        raise ValueError(f"{name} must have {numel} elements, got {t.numel()}")
+    raise ValueError(f"{name} must be contiguous")
+
+
+def _heads(t, dtype, name, index, shape=None):
+    """Address and row stride of a [rows, heads, 64] operand whose rows may be strided (a projection's columns)."""
+    if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.get_device() != index:
+        _wrong(t, dtype, name, index)
+    if t.dim() != 3 or t.shape[2] != 64 or (shape is not None and t.shape != shape):
         raise ValueError(f"{name} must be [rows, heads, 64]{'' if shape is None else f' = {list(shape)}'}, got {list(t.shape)}")
     rows, heads, _ = t.shape
-    if rows and heads and (t.stride(2) != 1 or (heads > 1 and t.stride(1) != 64)):
+    if t.is_contiguous():
+        return t.data_ptr(), heads * 64
+    if t.stride(2) != 1 or (heads > 1 and t.stride(1) != 64):
         raise ValueError(f"{name}: a row's heads and dims must be contiguous")
     return t.data_ptr(), (t.stride(0) if rows > 1 else heads * 64)
 
 
-def _vec(t, dtype, name, device, numel=None):
-    """Address of a contiguous operand on `device` (None passes through)."""
+def _vec(t, dtype, name, index, numel=None):
+    """Address of a contiguous operand on the device (None passes through)."""
     if t is None:
         return None
-    p = _dev(t, dtype, name)
-    if t.device != device:
-        raise ValueError(f"{name} is on {t.device}, not on {device}")
-    if numel is not None and t.numel() != numel:
-        raise ValueError(f"{name} must have {numel} elements, got {t.numel()}")
-    return p
+    if (not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.get_device() != index or not t.is_contiguous()
+            or (numel is not None and t.numel() != numel)):
+        _wrong(t, dtype, name, index, numel)
+    return t.data_ptr()
 
 
-def _pages(page_table, pool, page_bytes, layer, device):
+def _pages(page_table, pool, page_bytes, layer, index):
     """The cache arguments of the C entry points from the page table [slots, max_pages] on."""
-    table = _vec(page_table, torch.int32, "page_table", device)
-    if page_table.dim() != 2:
-        raise ValueError("page_table must be [slots, max_pages]")
-    bytes_ = _vec(pool, torch.uint8, "pool", device)
+    table, bytes_ = _vec(page_table, _I32, "page_table", index), _vec(pool, _U8, "pool", index)
+    if table is None or bytes_ is None or page_table.dim() != 2:
+        raise ValueError("page_table must be [slots, max_pages], and a pool is needed")
     if page_bytes <= 0:
         raise ValueError(f"page_bytes {page_bytes}")
     slots, max_pages = page_table.shape
     return table, slots, max_pages, bytes_, page_bytes, pool.numel() // page_bytes, layer
 
 
-def _call_on(device, name, *args):
+def _call_on(index, name, *args):
     """The call on the device's current stream (whichever device is current)."""
-    if device.index == torch.cuda.current_device():
-        return call(name, *args, _stream())
-    with torch.cuda.device(device):
-        return call(name, *args, _stream())
+    if index == torch.cuda.current_device():
+        return call(name, *args, torch._C._cuda_getCurrentRawStream(index))
+    with torch.cuda.device(index):
+        return call(name, *args, torch._C._cuda_getCurrentRawStream(index))
 
 
 def kv_append(k, v, row_slot, row_pos, page_table, pool, page_bytes, layer, status=None):
@@ -238,29 +253,31 @@ def kv_append(k, v, row_slot, row_pos, page_table, pool, page_bytes, layer, stat
     possibly strided; row_slot, row_pos int32 [rows] (distinct positions; a
     negative position: padding); page_table int32 [slots, max_pages], pool
     uint8 [num_pages * page_bytes]."""
-    code, device = _type(k, "k"), k.device
-    kp, ks = _heads(k, k.dtype, "k", device)
-    vp, vs = _heads(v, k.dtype, "v", device, k.shape)
+    code, index = _start(k, "k")
+    kp, ks = _heads(k, k.dtype, "k", index)
     rows, kv_heads, _ = k.shape
-    _call_on(device, "ndl_kv_append", kp, ks, vp, vs, code, _vec(row_slot, torch.int32, "row_slot", device, rows),
-             _vec(row_pos, torch.int32, "row_pos", device, rows), rows, kv_heads,
-             *_pages(page_table, pool, page_bytes, layer, device), _vec(status, torch.int32, "status", device))
+    vp, vs = _heads(v, k.dtype, "v", index, k.shape)
+    _call_on(index, "ndl_kv_append", kp, ks, vp, vs, code, _vec(row_slot, _I32, "row_slot", index, rows),
+             _vec(row_pos, _I32, "row_pos", index, rows), rows, kv_heads,
+             *_pages(page_table, pool, page_bytes, layer, index), _vec(status, _I32, "status", index))
 
 
 def kv_gather(row_slot, row_pos, kv_heads, page_table, pool, page_bytes, layer, dtype=torch.float32, k=None, v=None,
               status=None):
     """The values the pages hold for the rows (ndl_kv_gather): k and v
     [rows, kv_heads, 64] of `dtype` (or of the tensors given)."""
-    device, rows = pool.device, row_slot.numel()
-    k = torch.empty((rows, kv_heads, 64), dtype=dtype, device=device) if k is None else k
-    v = torch.empty((rows, kv_heads, 64), dtype=k.dtype, device=device) if v is None else v
-    code = _type(k, "k")
-    kp, ks = _heads(k, k.dtype, "k", device, (rows, kv_heads, 64))
-    vp, vs = _heads(v, k.dtype, "v", device, (rows, kv_heads, 64))
-    _call_on(device, "ndl_kv_gather", _vec(row_slot, torch.int32, "row_slot", device),
-             _vec(row_pos, torch.int32, "row_pos", device, rows), rows, kv_heads,
-             *_pages(page_table, pool, page_bytes, layer, device), kp, ks, vp, vs, code,
-             _vec(status, torch.int32, "status", device))
+    _, index = _start(pool, "pool", {_U8: 0})
+    rows = row_slot.numel()
+    shape = (rows, kv_heads, 64)
+    k = pool.new_empty(shape, dtype=dtype) if k is None else k
+    v = torch.empty_like(k, memory_format=torch.contiguous_format) if v is None else v
+    code, _ = _start(k, "k")
+    kp, ks = _heads(k, k.dtype, "k", index, shape)
+    vp, vs = _heads(v, k.dtype, "v", index, shape)
+    _call_on(index, "ndl_kv_gather", _vec(row_slot, _I32, "row_slot", index),
+             _vec(row_pos, _I32, "row_pos", index, rows), rows, kv_heads,
+             *_pages(page_table, pool, page_bytes, layer, index), kp, ks, vp, vs, code,
+             _vec(status, _I32, "status", index))
     return k, v
 
 
@@ -274,17 +291,16 @@ def attention_prompt(q, seq_rows, seq_slot, seq_pos, kv_heads, page_table, pool,
     of slot seq_slot[s], whose pages hold the keys and values up to the last
     of them.  window > 0: the last `window` positions only.  Rows of no
     sequence are left as they are in `out`."""
-    code, device = _type(q, "q"), q.device
-    qp, qs = _heads(q, q.dtype, "q", device)
-    out = torch.empty(q.shape, dtype=q.dtype, device=device) if out is None else out
-    op, os_ = _heads(out, q.dtype, "out", device, q.shape)
+    code, index = _start(q, "q")
+    qp, qs = _heads(q, q.dtype, "q", index)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format) if out is None else out
+    op, os_ = _heads(out, q.dtype, "out", index, q.shape)
     rows, heads, _ = q.shape
     sequences = seq_slot.numel()
-    _call_on(device, "ndl_attention_prompt", qp, qs, code,
-             _vec(seq_rows, torch.int32, "seq_rows", device, sequences + 1),
-             _vec(seq_slot, torch.int32, "seq_slot", device), _vec(seq_pos, torch.int32, "seq_pos", device, sequences),
-             sequences, rows, heads, kv_heads, scale, window, *_pages(page_table, pool, page_bytes, layer, device), op,
-             os_, _vec(status, torch.int32, "status", device))
+    _call_on(index, "ndl_attention_prompt", qp, qs, code, _vec(seq_rows, _I32, "seq_rows", index, sequences + 1),
+             _vec(seq_slot, _I32, "seq_slot", index), _vec(seq_pos, _I32, "seq_pos", index, sequences), sequences,
+             rows, heads, kv_heads, scale, window, *_pages(page_table, pool, page_bytes, layer, index), op, os_,
+             _vec(status, _I32, "status", index))
     return out
 
 
@@ -301,19 +317,17 @@ def attention_split(q, row_slot, row_len, kv_heads, page_table, pool, page_bytes
     `window` of them) of slot row_slot[r]; length 0 gives zeros.  workspace
     uint8 [attention_split_workspace(...)]: allocated for the call if none is
     given; calls that overlap need one each."""
-    code, device = _type(q, "q"), q.device
-    qp, qs = _heads(q, q.dtype, "q", device)
-    out = torch.empty(q.shape, dtype=q.dtype, device=device) if out is None else out
-    op, os_ = _heads(out, q.dtype, "out", device, q.shape)
+    code, index = _start(q, "q")
+    qp, qs = _heads(q, q.dtype, "q", index)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format) if out is None else out
+    op, os_ = _heads(out, q.dtype, "out", index, q.shape)
     rows, heads, _ = q.shape
-    pages = _pages(page_table, pool, page_bytes, layer, device)
+    pages = _pages(page_table, pool, page_bytes, layer, index)
     if workspace is None:
-        need = lib().ndl_attention_split_workspace(rows, heads, kv_heads, pages[2])
-        workspace = torch.empty(need, dtype=torch.uint8, device=device)
-    _call_on(device, "ndl_attention_split", qp, qs, code, _vec(row_slot, torch.int32, "row_slot", device, rows),
-             _vec(row_len, torch.int32, "row_len", device, rows), rows, heads, kv_heads, scale, window, *pages, op, os_,
-             _vec(workspace, torch.uint8, "workspace", device), workspace.numel(),
-             _vec(status, torch.int32, "status", device))
+        workspace = pool.new_empty(lib().ndl_attention_split_workspace(rows, heads, kv_heads, pages[2]))
+    _call_on(index, "ndl_attention_split", qp, qs, code, _vec(row_slot, _I32, "row_slot", index, rows),
+             _vec(row_len, _I32, "row_len", index, rows), rows, heads, kv_heads, scale, window, *pages, op, os_,
+             _vec(workspace, _U8, "workspace", index), workspace.numel(), _vec(status, _I32, "status", index))
     return out
 
 
@@ -328,29 +342,27 @@ def logits_process(logits, out=None, tokens=None, token_offsets=None, prompt_len
     [bias_offsets[r]:bias_offsets[r+1]]; mask int32 [mask rows, words] (bit
     set: allowed), row mask_index[r] of it (negative: none), without
     mask_index row r.  out may be `logits` itself."""
-    device = logits.device
+    _, index = _start(logits, "logits", {_F32: 0})
+    out = torch.empty_like(logits, memory_format=torch.contiguous_format) if out is None else out
     if logits.dim() != 2:
         raise ValueError("logits must be [rows, vocab]")
     rows, vocab = logits.shape
-    out = torch.empty((rows, vocab), dtype=torch.float32, device=device) if out is None else out
 
     def matrix(t, name):
-        if not t.is_cuda or t.dtype != torch.float32:
-            raise TypeError(f"{name} must be a float32 CUDA tensor")
-        if t.device != device or tuple(t.shape) != (rows, vocab) or (vocab > 1 and t.stride(1) != 1):
-            raise ValueError(f"{name} must be [{rows}, {vocab}] on {device} with contiguous rows")
+        if not isinstance(t, torch.Tensor) or t.dtype is not _F32 or t.get_device() != index:
+            _wrong(t, _F32, name, index)
+        if t.shape != logits.shape or (vocab > 1 and t.stride(1) != 1):
+            raise ValueError(f"{name} must be [{rows}, {vocab}] with contiguous rows")
         return t.data_ptr(), (t.stride(0) if rows > 1 else vocab)
 
-    i32, f32 = torch.int32, torch.float32
+    n_bias = 0 if bias_ids is None else bias_ids.numel()
     mask_rows, words = (0, 0) if mask is None else mask.shape
-    _call_on(device, "ndl_logits_process", *matrix(logits, "logits"), *matrix(out, "out"), rows, vocab,
-             _vec(tokens, i32, "tokens", device), 0 if tokens is None else tokens.numel(),
-             _vec(token_offsets, i32, "token_offsets", device, rows + 1),
-             _vec(prompt_lens, i32, "prompt_lens", device, rows), _vec(repetition, f32, "repetition", device, rows),
-             _vec(frequency, f32, "frequency", device, rows), _vec(presence, f32, "presence", device, rows),
-             _vec(bias_ids, i32, "bias_ids", device),
-             _vec(bias_values, f32, "bias_values", device, None if bias_ids is None else bias_ids.numel()),
-             0 if bias_ids is None else bias_ids.numel(), _vec(bias_offsets, i32, "bias_offsets", device, rows + 1),
-             _vec(mask, i32, "mask", device), mask_rows, words, _vec(mask_index, i32, "mask_index", device, rows),
-             _vec(status, i32, "status", device))
+    _call_on(index, "ndl_logits_process", *matrix(logits, "logits"), *matrix(out, "out"), rows, vocab,
+             _vec(tokens, _I32, "tokens", index), 0 if tokens is None else tokens.numel(),
+             _vec(token_offsets, _I32, "token_offsets", index, rows + 1),
+             _vec(prompt_lens, _I32, "prompt_lens", index, rows), _vec(repetition, _F32, "repetition", index, rows),
+             _vec(frequency, _F32, "frequency", index, rows), _vec(presence, _F32, "presence", index, rows),
+             _vec(bias_ids, _I32, "bias_ids", index), _vec(bias_values, _F32, "bias_values", index, n_bias), n_bias,
+             _vec(bias_offsets, _I32, "bias_offsets", index, rows + 1), _vec(mask, _I32, "mask", index), mask_rows,
+             words, _vec(mask_index, _I32, "mask_index", index, rows), _vec(status, _I32, "status", index))
     return out

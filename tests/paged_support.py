@@ -96,11 +96,17 @@ def bound(kind, out, size, reach, count, largest):
     - exp adds 2^-21, a probability rounds by half a step of fp16 (2^-11) for
       16-bit types, for fp32 it is two halves (2^-21); both the sum over v and
       the total carry the factor, the sums themselves round within 2^-18;
+    - bf16 callers of the prompt get keys and values as code * scale in fp16:
+      a key element is off by two roundings of the product (2 * 2^-11), so a
+      score by 2^-10 * reach, a value by its scale's rounding and the
+      product's (2 * 2^-11);
     - below fp16's normal range a probability is off by 2^-25 of one that is
       at least 2^-1 (fp32: 2^-36, the second half's);
     - the result rounds by half a step of its type."""
     d = 72 * 2.0 ** -23 * (2 * reach[:, None] + 1)
-    p = 2.0 ** -21 if kind == "f32" else 2.0 ** -11
+    p = {"f32": 2.0 ** -21, "f16": 2.0 ** -11, "bf16": 3 * 2.0 ** -11}[kind]
+    if kind == "bf16":
+        d = d + 2 * 2.0 ** -10 * reach[:, None]
     tiny = (2.0 ** -35 if kind == "f32" else 2.0 ** -24) * count * largest
     return size * (2 * (np.expm1(d) + 2.0 ** -21) + p + 2.0 ** -18) + tiny + HALF_STEP[kind] * (np.abs(out) + 1e-30)
 
