@@ -34,8 +34,6 @@
 // scale by NaN, which only the rows that see the position take up.
 #include <float.h>
 
-#include <type_traits>
-
 #include "attention_math.cuh"
 #include "tc.cuh"
 
@@ -43,34 +41,36 @@ namespace ndl {
 
 namespace {
 
-constexpr int kTileRows = 128;                 // MMA rows: TMEM lanes
-constexpr int kCtaRows = 2 * kTileRows;
-constexpr int kConvertWarp = 8, kConvertWarps = 4, kMmaWarp = 12, kCopyWarp = 13;
-constexpr int kPromptThreads = 16 * 32;
-// Registers a thread: 128 at launch (512 threads); the softmax warps, which hold 128 scores a row, take over what the
-// converters and the last warpgroup (MMA and copies) give up: 2 * 184 + 96 + 48 = 4 * 128.
-constexpr int kSoftmaxRegs = 184, kConvertRegs = 96, kMmaRegs = 48;
-static_assert(2 * kSoftmaxRegs + kConvertRegs + kMmaRegs == 4 * 128, "the launch's registers, shared out");
+constexpr int kTileRows = 128;  // MMA rows: TMEM lanes
 constexpr int kTileBytes = kTileRows * kHeadDim * 2;      // 16 KB of queries
 constexpr int kPageTile = kPagePositions * kHeadDim * 2;  // 8 KB of keys or values
-constexpr uint32_t kPromptWait = 1u << 22;     // waits of about a microsecond: a few seconds
+constexpr uint32_t kPromptWait = 1u << 22;                // waits of about a microsecond: a few seconds
 constexpr int kTmemCols = 512;
-constexpr int kStagger = 4;                    // steps from which the tiles run half a step apart
+constexpr int kConvertWarps = 4;
 
-// The forms of the element types (above).  The second parts of fp32 leave
-// TMEM room for one page a step.
+// The forms of the element types (above).
 template <class T>
 struct Step {
     static constexpr bool kSplit = sizeof(T) == 4;                       // queries and P in two parts
     static constexpr bool kFoldValues = __is_same(T, __nv_bfloat16);     // value scales on the values, else on P
     static constexpr int kQParts = kSplit ? 2 : 1, kKParts = kFoldValues ? 1 : 2;
-    static constexpr int kPages = kSplit ? 1 : 2, kCols = kPages * kPagePositions;
-    static constexpr int kStages = kSplit ? 4 : 3;  // converted steps in flight
-    static constexpr int kRaw = 2;                  // steps of records as they lie in the pages
-    // TMEM columns: scores, outputs, probabilities (two fp16 a column; fp32: then their second parts) of both tiles
-    static constexpr int kS = 0, kO = 2 * kCols, kP = kO + 2 * kHeadDim, kPCols = kCols / 2;
-    static constexpr int kLo = 2 * kPCols;
-    static_assert(kP + 2 * kPCols * (kSplit ? 2 : 1) <= kTmemCols, "TMEM columns");
+    // Tiles of 128 rows: three, whose softmax warps pass their waits under one another's exponentials; the second
+    // parts of fp32 leave TMEM room for two.
+    static constexpr int kTiles = kSplit ? 2 : 3, kRows = kTiles * kTileRows;
+    static constexpr int kPages = 1, kCols = kPages * kPagePositions;
+    static constexpr int kStages = 4;  // converted steps in flight
+    static constexpr int kRaw = 3;     // steps of records as they lie in the pages
+    // TMEM columns: scores, outputs, probabilities (two fp16 a column; fp32: then their second parts) of the tiles
+    static constexpr int kS = 0, kO = kTiles * kCols, kP = kO + kTiles * kHeadDim, kPCols = kCols / 2;
+    static constexpr int kLo = kTiles * kPCols;
+    static_assert(kP + kTiles * kPCols * (kSplit ? 2 : 1) <= kTmemCols, "TMEM columns");
+    // Warps: softmax, converters, then a group of one MMA warp a tile and one that copies.
+    static constexpr int kConvertWarp = 4 * kTiles, kMmaWarp = kConvertWarp + kConvertWarps, kCopyWarp = kMmaWarp + 3;
+    static constexpr int kThreads = 32 * (kMmaWarp + 4);
+    // Registers a thread: what the launch gives each (128 or 96), shared out anew: the softmax warps hold a row's scores.
+    static constexpr int kLaunchRegs = kTiles == 2 ? 128 : 96;
+    static constexpr int kSoftmaxRegs = kTiles == 2 ? 184 : 120, kConvertRegs = kTiles == 2 ? 96 : 72, kMmaRegs = 48;
+    static_assert(kTiles * kSoftmaxRegs + kConvertRegs + kMmaRegs == (kTiles + 2) * kLaunchRegs, "the launch's registers");
 };
 
 struct PromptArgs {
@@ -86,7 +86,7 @@ struct PromptArgs {
 template <class T>
 struct PromptSmem {
     using St = Step<T>;
-    uint8_t q[2][St::kQParts][kTileBytes];  // 1024-byte aligned
+    uint8_t q[St::kTiles][St::kQParts][kTileBytes];  // 1024-byte aligned
     uint8_t k[St::kStages][St::kKParts][St::kPages][kPageTile], v[St::kStages][St::kPages][kPageTile];
     uint8_t raw[St::kRaw][St::kPages][kKvBlockBytes];
     float scales[kConvertWarps][2][St::kPages][kPagePositions];  // each converter warp's copy: keys, values
@@ -95,9 +95,9 @@ struct PromptSmem {
     int exponent[St::kStages];      // of the value scales so far
     uint64_t raw_full[St::kRaw], kv_full[St::kStages], kv_empty[St::kStages];
     int missing[St::kRaw];  // bit g: the step's page g is not in the pool
-    uint64_t s_full[2], s_free[2], p_full[2], pv_done[2];
+    uint64_t s_full[St::kTiles], s_free[St::kTiles], p_full[St::kTiles], pv_done[St::kTiles];
     uint32_t tmem;
-    int seq, tile;  // this CTA's work: sequence (-1: none) and 256-row tile of it
+    int seq, tile;  // this CTA's work: sequence (-1: none) and the kRows-row tile of it
     volatile int abort;
 };
 
@@ -135,10 +135,11 @@ __device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity, volati
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 template <class T>
-__global__ void __launch_bounds__(kPromptThreads, 1) attention_prompt_kernel(PromptArgs a) {
+__global__ void __launch_bounds__(Step<T>::kThreads, 1) attention_prompt_kernel(PromptArgs a) {
     using St = Step<T>;
     constexpr bool kSplit = St::kSplit;
-    constexpr int kStages = St::kStages, kPages = St::kPages, kCols = St::kCols;
+    constexpr int kStages = St::kStages, kPages = St::kPages, kCols = St::kCols, kTiles = St::kTiles;
+    constexpr int kCtaRows = St::kRows, kMmaWarp = St::kMmaWarp;
     extern __shared__ uint8_t smem_raw[];
     PromptSmem<T> &s =
         *reinterpret_cast<PromptSmem<T> *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -146,7 +147,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attention_prompt_kernel(Pro
     const int kv_head = blockIdx.x % a.c.heads, work = blockIdx.x / a.c.heads;
     const int group = a.heads / a.c.heads;
 
-    // This CTA's tile: sequences hold ceil(rows * group / 256) tiles each.
+    // This CTA's tile: sequences hold ceil(rows * group / kCtaRows) tiles each.
     if (warp == 0) {
         int seq = -1, tile = 0, before = 0;
         for (int base = 0; base < a.sequences && seq < 0; base += 32) {
@@ -181,8 +182,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attention_prompt_kernel(Pro
     } else if (warp == kMmaWarp) {
         if (lane == 0) {
             for (int i = 0; i < St::kRaw; i++) mbar_init(&s.raw_full[i], 1);
-            for (int i = 0; i < kStages; i++) mbar_init(&s.kv_full[i], kConvertWarps), mbar_init(&s.kv_empty[i], 2);
-            for (int t = 0; t < 2; t++)
+            for (int i = 0; i < kStages; i++) mbar_init(&s.kv_full[i], kConvertWarps), mbar_init(&s.kv_empty[i], kTiles);
+            for (int t = 0; t < kTiles; t++)
                 mbar_init(&s.s_full[t], 1), mbar_init(&s.s_free[t], 4), mbar_init(&s.p_full[t], 4),
                     mbar_init(&s.pv_done[t], 1);
             fence_mbar_init();
@@ -203,9 +204,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attention_prompt_kernel(Pro
                         (long long)start + n <= (long long)a.c.max_pages * kPagePositions;
     const long long packed = (long long)n * group, m0 = (long long)s.tile * kCtaRows;
     // the pages its rows see, from page0 on in steps; steps [lo, hi] of each tile (hi < lo: no rows)
-    int lo[2], hi[2], page0 = 0;
+    int lo[kTiles], hi[kTiles], page0 = 0, steps = 0;
 #pragma unroll
-    for (int t = 0; t < 2; t++) {
+    for (int t = 0; t < kTiles; t++) {
         const long long b = m0 + t * kTileRows, e = min(packed, b + kTileRows);
         lo[t] = 0, hi[t] = -1;
         if (seq >= 0 && ok_seq && b < e) {
@@ -214,22 +215,25 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attention_prompt_kernel(Pro
             if (t == 0) page0 = first;
             lo[t] = (first - page0) / kPages;
             hi[t] = (to / kPagePositions - page0) / kPages;
+            steps = max(steps, hi[t] + 1);
         }
     }
-    const int steps = max(hi[0], hi[1]) + 1;
+    // a warp's tile, and the steps it takes
+    const auto pick = [&](const int(&x)[kTiles], int t) { return t == 0 ? x[0] : t == 1 ? x[1] : x[kTiles - 1]; };
     const int last_pos = start + (int)((min(packed, m0 + kCtaRows) - 1) / group);  // the CTA's last query
 
-    if (warp < kConvertWarp) {
+    if (warp < St::kConvertWarp) {
         // ------------------------------------------------------- softmax --
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(St::kSoftmaxRegs));
         const int t = warp >> 2, row = threadIdx.x & (kTileRows - 1);
+        const int lo_t = pick(lo, t), hi_t = pick(hi, t);
         const long long m = m0 + t * kTileRows + row;
         const bool valid = seq >= 0 && m < packed;
         const int query = valid ? (int)(m / group) : 0, head = kv_head * group + (valid ? (int)(m % group) : 0);
         const size_t at = (size_t)(first_row + query);
         const int pos = start + query;
         float scale_q = 1.0f;
-        if (hi[t] >= lo[t]) {
+        if (hi_t >= lo_t) {
             // the query row: normalised to fp16 (in two parts), dims in the
             // order the key tiles have them, into the swizzled A tile
             const T *src = static_cast<const T *>(a.q) + at * a.q_stride + (size_t)head * kHeadDim;
@@ -266,66 +270,64 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attention_prompt_kernel(Pro
         float top = -INFINITY, total = 0.0f;
         int exponent = kMinExponent;
         bool ok = true;
-        for (int i = lo[t]; i <= hi[t]; i++) {
-            const int it = i - lo[t], st = i % kStages;
-            ok = warp_wait(&s.s_full[t], it & 1, &s.abort) && warp_wait(&s.kv_full[st], (i / kStages) & 1, &s.abort);
+        // Tests of barriers are made ahead of their use: one takes some 70 clocks to answer, a vote on it 40.
+        bool kv_ready = false;
+        for (int i = lo_t; i <= hi_t; i++) {
+            const int it = i - lo_t, st = i % kStages;
+            if (!__all_sync(0xffffffffu, kv_ready)) ok = warp_wait(&s.kv_full[st], (i / kStages) & 1, &s.abort);
+            ok = ok && warp_wait(&s.s_full[t], it & 1, &s.abort);
             if (!ok) break;
             tc_fence_after();
             uint32_t r[kCols];
 #pragma unroll
             for (int c = 0; c < kCols; c += 32) tmem_ld32(ts + c, reinterpret_cast<uint32_t(&)[32]>(r[c]));
-            tmem_ld_wait(r);
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&s.s_free[t]);
+            const bool pv_ready = it == 0 || mbar_test_wait(&s.pv_done[t], (it - 1) & 1);
+            const int ke = s.exponent[st];
+            const float f = fminf(fmaxf(scale_q * s.key_factor[st], FLT_MIN), FLT_MAX);  // it multiplies infinities
             // positions [from, upto] of the step are this row's
             const int upto = pos - (page0 + i * kPages) * kPagePositions;
             const int from = a.window ? upto - a.window + 1 : 0;
             const bool whole = __all_sync(0xffffffffu, upto >= kCols - 1 && from <= 0);
-            const int ke = s.exponent[st];
-            const float f = fminf(fmaxf(scale_q * s.key_factor[st], FLT_MIN), FLT_MAX);  // it multiplies infinities
-            // two copies, so that steps every row sees whole carry no masks
-            const auto step = [&](auto masked) {
-                if constexpr (decltype(masked)::value) {
+            tmem_ld_wait(r);
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&s.s_free[t]);
+            if (!whole) {
 #pragma unroll
-                    for (int j = 0; j < kCols; j++)
-                        if (j > upto || j < from) r[j] = __float_as_uint(-INFINITY);
+                for (int j = 0; j < kCols; j++)
+                    if (j > upto || j < from) r[j] = __float_as_uint(-INFINITY);
+            }
+            // the previous product has read P and finished O
+            if (!__all_sync(0xffffffffu, pv_ready)) {
+                ok = warp_wait(&s.pv_done[t], (it - 1) & 1, &s.abort);
+                if (!ok) break;
+            }
+            tc_fence_after();
+            kv_ready = mbar_test_wait(&s.kv_full[(i + 1) % kStages], ((i + 1) / kStages) & 1);
+            const auto rescale = [&](float keep) {  // O of the earlier steps
+                if (it == 0 || !__any_sync(0xffffffffu, keep != 1.0f)) return;
+#pragma unroll
+                for (int c = 0; c < kHeadDim; c += 16) {
+                    uint32_t o[16];
+                    tmem_ld16(to + c, o);
+                    tmem_ld_wait(o);
+#pragma unroll
+                    for (int j = 0; j < 16; j++) o[j] = __float_as_uint(__uint_as_float(o[j]) * keep);
+                    tmem_st16(to + c, o);
                 }
-                float peaks[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                for (int j = 0; j < kCols; j += 2)
-                    peaks[(j >> 1) & 3] = fmaxf(peaks[(j >> 1) & 3], fmaxf(__uint_as_float(r[j]), __uint_as_float(r[j + 1])));
-                const float peak = fmaxf(fmaxf(peaks[0], peaks[1]), fmaxf(peaks[2], peaks[3])) * f;
-                float keep = 1.0f;
-                if (peak - top > kLazy || (top == -INFINITY && peak > -INFINITY)) {
-                    keep = top == -INFINITY ? 0.0f : exp2_approx(top - peak);
-                    total *= keep;
-                    top = peak;
-                }
-                if (ke > exponent) keep *= exp2_approx((float)(exponent - ke));
-                exponent = ke;
-                // the previous product has read P and finished O
-                if (it > 0) {
-                    ok = warp_wait(&s.pv_done[t], (it - 1) & 1, &s.abort);
-                    if (!ok) return;
-                    tc_fence_after();
-                    if (__any_sync(0xffffffffu, keep != 1.0f)) {
-#pragma unroll
-                        for (int c = 0; c < kHeadDim; c += 16) {
-                            uint32_t o[16];
-                            tmem_ld16(to + c, o);
-                            tmem_ld_wait(o);
-#pragma unroll
-                            for (int j = 0; j < 16; j++) o[j] = __float_as_uint(__uint_as_float(o[j]) * keep);
-                            tmem_st16(to + c, o);
-                        }
-                    }
-                }
+            };
+            if (ke > exponent) rescale(exp2_approx((float)(exponent - ke)));
+            exponent = ke;
+            // P with the maximum as it stands, the step's own found beside it: the exponential unit bounds this loop, and
+            // the step is done again where the maximum has to move (the first steps, hardly any later).
+            float step_sum;
+            for (int pass = 0;; pass++) {
                 // folded value scales leave P room up to 2^15
                 const float base = (top == -INFINITY ? 0.0f : top) - (St::kFoldValues ? 8.0f : 0.0f);
                 [[maybe_unused]] const ulonglong2 *vs = reinterpret_cast<const ulonglong2 *>(s.vs[st]);
                 const uint64_t f2 = f2_pack(f, f), base2 = f2_pack(-base, -base);
                 uint64_t sums[2] = {0, 0};
+                float peaks[2] = {-INFINITY, -INFINITY};
 #pragma unroll
                 for (int c = 0; c < kCols; c += 32) {
                     uint32_t hp[16];
@@ -337,8 +339,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attention_prompt_kernel(Pro
 #pragma unroll
                         for (int u = 0; u < 2; u++) {
                             const int k = c + j + 2 * u;
+                            const float x0 = __uint_as_float(r[k]), x1 = __uint_as_float(r[k + 1]);
+                            peaks[u] = fmaxf(peaks[u], fmaxf(x0, x1));
                             float e0, e1;
-                            f2_unpack(f2_fma(f2_pack(__uint_as_float(r[k]), __uint_as_float(r[k + 1])), f2, base2), e0, e1);
+                            f2_unpack(f2_fma(f2_pack(x0, x1), f2, base2), e0, e1);
                             e0 = exp2_approx(e0), e1 = exp2_approx(e1);
                             const uint64_t e = f2_pack(e0, e1);
                             sums[u] = f2_add(sums[u], e);
@@ -352,19 +356,27 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attention_prompt_kernel(Pro
                 }
                 float sum0, sum1;
                 f2_unpack(f2_add(sums[0], sums[1]), sum0, sum1);
-                total += sum0 + sum1;
-            };
-            if (whole) step(std::false_type{});
-            else step(std::true_type{});
-            if (!ok) break;
+                step_sum = sum0 + sum1;
+                const float peak = fmaxf(peaks[0], peaks[1]) * f;
+                const bool moves = peak - top > kLazy || (top == -INFINITY && peak > -INFINITY);
+                if (pass > 0 || !__any_sync(0xffffffffu, moves)) break;
+                float keep = 1.0f;
+                if (moves) {
+                    keep = top == -INFINITY ? 0.0f : exp2_approx(top - peak);
+                    total *= keep;
+                    top = peak;
+                }
+                rescale(keep);
+            }
+            total += step_sum;
             tmem_st_wait();
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&s.p_full[t]);
         }
         // the rows' results
-        if (hi[t] >= lo[t]) {
-            ok = ok && warp_wait(&s.pv_done[t], (hi[t] - lo[t]) & 1, &s.abort);
+        if (hi_t >= lo_t) {
+            ok = ok && warp_wait(&s.pv_done[t], (hi_t - lo_t) & 1, &s.abort);
             if (!ok) {
                 s.abort = 1;
                 if (lane == 0 && a.c.status) atomicOr(a.c.status, kStatusTimeout);
@@ -398,8 +410,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attention_prompt_kernel(Pro
         }
     } else if (warp < kMmaWarp) {
         // -------------------------------------------------- page converter --
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kConvertRegs));
-        const int c = warp - kConvertWarp;
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(St::kConvertRegs));
+        const int c = warp - St::kConvertWarp;
         int exponent = kMinExponent;
         const float fold = a.scale * kLog2E;
         __syncthreads();
@@ -517,10 +529,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attention_prompt_kernel(Pro
         }
     } else {
         // ------------------------------------------------------ MMA issuer --
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kMmaRegs));
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(St::kMmaRegs));
         __syncthreads();
         bool ok = true;
-        if (warp == kCopyWarp) {
+        if (warp == St::kCopyWarp) {
             // the records of each step into their ring, once the converters have read the step kRaw before
             const int page_end = last_pos / kPagePositions + 1;
             int ids = -1, i = 0;
@@ -555,14 +567,14 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attention_prompt_kernel(Pro
             if (!ok)
                 for (int j = max(0, i - St::kRaw); j < i; j++)
                     mbar_wait_bounded(&s.raw_full[j % St::kRaw], (j / St::kRaw) & 1, kPromptWait);
-        } else if (warp == kMmaWarp || warp == kMmaWarp + 2) {
+        } else if (warp < kMmaWarp + kTiles) {
             // A warp issues the products of one tile.
             constexpr uint32_t idesc_s = idesc_f16(kTileRows, kCols), idesc_o = idesc_f16(kTileRows, kHeadDim);
-            const int t = (warp - kMmaWarp) >> 1;
+            const int t = warp - kMmaWarp, lo_t = pick(lo, t), hi_t = pick(hi, t);
             const uint32_t ts = tmem + St::kS + t * kCols, to = tmem + St::kO + t * kHeadDim, tp = tmem + St::kP + t * St::kPCols;
             auto scores = [&](int i) {
-                if (!ok || i < lo[t] || i > hi[t]) return;
-                const int it = i - lo[t], st = i % kStages;
+                if (!ok || i < lo_t || i > hi_t) return;
+                const int it = i - lo_t, st = i % kStages;
                 ok = warp_wait(&s.kv_full[st], (i / kStages) & 1, &s.abort) &&
                      (it == 0 || warp_wait(&s.s_free[t], (it - 1) & 1, &s.abort));
                 if (!ok) return;
@@ -577,14 +589,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attention_prompt_kernel(Pro
                     }
                 mma_commit_elect(&s.s_full[t]);
             };
-            // The tiles run half a step apart, so that one's maxima and waits pass under the other's exponentials: tile
-            // 1 begins when tile 0 has its first probabilities.
-            if (t == 1 && steps >= kStagger) ok = warp_wait(&s.p_full[0], 0, &s.abort);
             scores(0);
             for (int i = 0; i < steps && ok; i++) {
                 scores(i + 1);
-                const int it = i - lo[t], st = i % kStages;
-                if (i >= lo[t] && i <= hi[t]) {
+                const int it = i - lo_t, st = i % kStages;
+                if (i >= lo_t && i <= hi_t) {
                     ok = ok && warp_wait(&s.p_full[t], it & 1, &s.abort);
                     if (!ok) break;
                     tc_fence_after();
@@ -595,7 +604,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attention_prompt_kernel(Pro
                             mma_f16_ts(to, tp + part * St::kLo + k * 8, sw128_kmajor_desc(s.v[st][k >> 2]) + 2 * (k & 3), idesc_o,
                                        it + part + k > 0);
                     mma_commit_elect(&s.pv_done[t]);
-                } else {  // the step is the other tile's alone
+                } else {  // the step is other tiles' alone
                     ok = warp_wait(&s.kv_full[st], (i / kStages) & 1, &s.abort);
                     if (!ok) break;
                 }
@@ -637,13 +646,13 @@ extern "C" NDL_API int ndl_attention_prompt(const void *q, long long q_stride, i
     PromptArgs a{q, out, q_stride, out_stride, seq_rows, seq_slot, seq_pos, rows, sequences, heads, window, scale,
                  {page_table, const_cast<uint8_t *>(pool), (long long)page_bytes, slots, max_pages, num_pages, layer,
                   kv_heads, status}};
-    // each sequence ends one tile early at most: no more tiles than these, whatever the lengths are
-    const long long tiles = (long long)rows * (heads / kv_heads) / kCtaRows + sequences;
-    NDL_REQUIRE(tiles * kv_heads <= 0x7FFFFFFFLL, "%d rows of %d heads in %d sequences: too many", rows, heads,
-                sequences);
     return with_type(type, [&](auto t) {
         using T = decltype(t);
         const auto kernel = attention_prompt_kernel<T>;
+        // each sequence ends one tile early at most: no more tiles than these, whatever the lengths are
+        const long long tiles = (long long)rows * (heads / kv_heads) / Step<T>::kRows + sequences;
+        NDL_REQUIRE(tiles * kv_heads <= 0x7FFFFFFFLL, "%d rows of %d heads in %d sequences: too many", rows, heads,
+                    sequences);
         constexpr size_t smem = sizeof(PromptSmem<T>) + 1024;
         static DeviceOnce attribute;  // the attribute belongs to the kernel on one device
         const int st = attribute.run([&] {
@@ -652,7 +661,7 @@ extern "C" NDL_API int ndl_attention_prompt(const void *q, long long q_stride, i
                                     : set_error(NDL_ERR_CUDA, "prompt attention smem: %s", cudaGetErrorString(e));
         });
         if (st != NDL_OK) return st;
-        kernel<<<(unsigned)(tiles * kv_heads), kPromptThreads, smem, (cudaStream_t)stream>>>(a);
+        kernel<<<(unsigned)(tiles * kv_heads), Step<T>::kThreads, smem, (cudaStream_t)stream>>>(a);
         return check_launch("attention_prompt");
     });
 }
