@@ -184,7 +184,7 @@ __global__ void __launch_bounds__(Step<T>::kThreads, 1) attention_prompt_kernel(
             for (int i = 0; i < St::kRaw; i++) mbar_init(&s.raw_full[i], 1);
             for (int i = 0; i < kStages; i++) mbar_init(&s.kv_full[i], kConvertWarps), mbar_init(&s.kv_empty[i], kTiles);
             for (int t = 0; t < kTiles; t++)
-                mbar_init(&s.s_full[t], 1), mbar_init(&s.s_free[t], 4), mbar_init(&s.p_full[t], 4),
+                mbar_init(&s.s_full[t], 2), mbar_init(&s.s_free[t], 4), mbar_init(&s.p_full[t], 4),
                     mbar_init(&s.pv_done[t], 1);
             fence_mbar_init();
         }
@@ -270,42 +270,77 @@ __global__ void __launch_bounds__(Step<T>::kThreads, 1) attention_prompt_kernel(
         float top = -INFINITY, total = 0.0f;
         int exponent = kMinExponent;
         bool ok = true;
-        // Tests of barriers are made ahead of their use: one takes some 70 clocks to answer, a vote on it 40.
-        bool kv_ready = false;
         for (int i = lo_t; i <= hi_t; i++) {
             const int it = i - lo_t, st = i % kStages;
-            if (!__all_sync(0xffffffffu, kv_ready)) ok = warp_wait(&s.kv_full[st], (i / kStages) & 1, &s.abort);
-            ok = ok && warp_wait(&s.s_full[t], it & 1, &s.abort);
+            // positions [from, upto] of the step are this row's
+            const int upto = pos - (page0 + i * kPages) * kPagePositions;
+            const int from = a.window ? upto - a.window + 1 : 0;
+            const bool whole = __all_sync(0xffffffffu, upto >= kCols - 1 && from <= 0);
+            ok = warp_wait(&s.s_full[t], it & 1, &s.abort);
             if (!ok) break;
             tc_fence_after();
             uint32_t r[kCols];
 #pragma unroll
             for (int c = 0; c < kCols; c += 32) tmem_ld32(ts + c, reinterpret_cast<uint32_t(&)[32]>(r[c]));
-            const bool pv_ready = it == 0 || mbar_test_wait(&s.pv_done[t], (it - 1) & 1);
             const int ke = s.exponent[st];
             const float f = fminf(fmaxf(scale_q * s.key_factor[st], FLT_MIN), FLT_MAX);  // it multiplies infinities
-            // positions [from, upto] of the step are this row's
-            const int upto = pos - (page0 + i * kPages) * kPagePositions;
-            const int from = a.window ? upto - a.window + 1 : 0;
-            const bool whole = __all_sync(0xffffffffu, upto >= kCols - 1 && from <= 0);
             tmem_ld_wait(r);
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&s.s_free[t]);
+            // has the previous product read P and finished O?  (asked ahead: the answer takes some 70 clocks)
+            const bool pv_ready = it == 0 || mbar_test_wait(&s.pv_done[t], (it - 1) & 1);
             if (!whole) {
 #pragma unroll
                 for (int j = 0; j < kCols; j++)
                     if (j > upto || j < from) r[j] = __float_as_uint(-INFINITY);
             }
-            // the previous product has read P and finished O
+            float peaks[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int j = 0; j < kCols; j += 2)
+                peaks[(j >> 1) & 3] = fmaxf(peaks[(j >> 1) & 3], fmaxf(__uint_as_float(r[j]), __uint_as_float(r[j + 1])));
+            const float peak = fmaxf(fmaxf(peaks[0], peaks[1]), fmaxf(peaks[2], peaks[3])) * f;
+            float keep = 1.0f;
+            if (peak - top > kLazy || (top == -INFINITY && peak > -INFINITY)) {
+                keep = top == -INFINITY ? 0.0f : exp2_approx(top - peak);
+                total *= keep;
+                top = peak;
+            }
+            if (ke > exponent) keep *= exp2_approx((float)(exponent - ke));
+            exponent = ke;
+            // folded value scales leave P room up to 2^15
+            const float base = (top == -INFINITY ? 0.0f : top) - (St::kFoldValues ? 8.0f : 0.0f);
+            [[maybe_unused]] const ulonglong2 *vs = reinterpret_cast<const ulonglong2 *>(s.vs[st]);
+            const uint64_t f2 = f2_pack(f, f), base2 = f2_pack(-base, -base);
+            uint64_t sums[2] = {0, 0};
+            uint32_t hp[kCols / 2];
+            [[maybe_unused]] uint32_t lp[kSplit ? kCols / 2 : 1];
+#pragma unroll
+            for (int j = 0; j < kCols; j += 4) {
+                [[maybe_unused]] ulonglong2 v2;
+                if constexpr (!St::kFoldValues) v2 = vs[j / 4];
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    const int k = j + 2 * u;
+                    float e0, e1;
+                    f2_unpack(f2_fma(f2_pack(__uint_as_float(r[k]), __uint_as_float(r[k + 1])), f2, base2), e0, e1);
+                    e0 = exp2_approx(e0), e1 = exp2_approx(e1);
+                    const uint64_t e = f2_pack(e0, e1);
+                    sums[u] = f2_add(sums[u], e);
+                    if constexpr (!St::kFoldValues) f2_unpack(f2_mul(e, u ? v2.y : v2.x), e0, e1);
+                    hp[k / 2] = half_pair(e0, e1);
+                    if constexpr (kSplit) lp[kSplit ? k / 2 : 0] = half_rest(e0, e1, hp[k / 2]);
+                }
+            }
+            float sum0, sum1;
+            f2_unpack(f2_add(sums[0], sums[1]), sum0, sum1);
+            total += sum0 + sum1;
             if (!__all_sync(0xffffffffu, pv_ready)) {
                 ok = warp_wait(&s.pv_done[t], (it - 1) & 1, &s.abort);
                 if (!ok) break;
             }
             tc_fence_after();
-            kv_ready = mbar_test_wait(&s.kv_full[(i + 1) % kStages], ((i + 1) / kStages) & 1);
-            const auto rescale = [&](float keep) {  // O of the earlier steps
-                if (it == 0 || !__any_sync(0xffffffffu, keep != 1.0f)) return;
+            if (it > 0 && __any_sync(0xffffffffu, keep != 1.0f)) {
 #pragma unroll
                 for (int c = 0; c < kHeadDim; c += 16) {
                     uint32_t o[16];
@@ -315,60 +350,12 @@ __global__ void __launch_bounds__(Step<T>::kThreads, 1) attention_prompt_kernel(
                     for (int j = 0; j < 16; j++) o[j] = __float_as_uint(__uint_as_float(o[j]) * keep);
                     tmem_st16(to + c, o);
                 }
-            };
-            if (ke > exponent) rescale(exp2_approx((float)(exponent - ke)));
-            exponent = ke;
-            // P with the maximum as it stands, the step's own found beside it: the exponential unit bounds this loop, and
-            // the step is done again where the maximum has to move (the first steps, hardly any later).
-            float step_sum;
-            for (int pass = 0;; pass++) {
-                // folded value scales leave P room up to 2^15
-                const float base = (top == -INFINITY ? 0.0f : top) - (St::kFoldValues ? 8.0f : 0.0f);
-                [[maybe_unused]] const ulonglong2 *vs = reinterpret_cast<const ulonglong2 *>(s.vs[st]);
-                const uint64_t f2 = f2_pack(f, f), base2 = f2_pack(-base, -base);
-                uint64_t sums[2] = {0, 0};
-                float peaks[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-                for (int c = 0; c < kCols; c += 32) {
-                    uint32_t hp[16];
-                    [[maybe_unused]] uint32_t lp[kSplit ? 16 : 1];
-#pragma unroll
-                    for (int j = 0; j < 32; j += 4) {
-                        [[maybe_unused]] ulonglong2 v2;
-                        if constexpr (!St::kFoldValues) v2 = vs[(c + j) / 4];
-#pragma unroll
-                        for (int u = 0; u < 2; u++) {
-                            const int k = c + j + 2 * u;
-                            const float x0 = __uint_as_float(r[k]), x1 = __uint_as_float(r[k + 1]);
-                            peaks[u] = fmaxf(peaks[u], fmaxf(x0, x1));
-                            float e0, e1;
-                            f2_unpack(f2_fma(f2_pack(x0, x1), f2, base2), e0, e1);
-                            e0 = exp2_approx(e0), e1 = exp2_approx(e1);
-                            const uint64_t e = f2_pack(e0, e1);
-                            sums[u] = f2_add(sums[u], e);
-                            if constexpr (!St::kFoldValues) f2_unpack(f2_mul(e, u ? v2.y : v2.x), e0, e1);
-                            hp[j / 2 + u] = half_pair(e0, e1);
-                            if constexpr (kSplit) lp[kSplit ? j / 2 + u : 0] = half_rest(e0, e1, hp[j / 2 + u]);
-                        }
-                    }
-                    tmem_st16(tp + c / 2, hp);
-                    if constexpr (kSplit) tmem_st16(tp + St::kLo + c / 2, reinterpret_cast<const uint32_t(&)[16]>(lp));
-                }
-                float sum0, sum1;
-                f2_unpack(f2_add(sums[0], sums[1]), sum0, sum1);
-                step_sum = sum0 + sum1;
-                const float peak = fmaxf(peaks[0], peaks[1]) * f;
-                const bool moves = peak - top > kLazy || (top == -INFINITY && peak > -INFINITY);
-                if (pass > 0 || !__any_sync(0xffffffffu, moves)) break;
-                float keep = 1.0f;
-                if (moves) {
-                    keep = top == -INFINITY ? 0.0f : exp2_approx(top - peak);
-                    total *= keep;
-                    top = peak;
-                }
-                rescale(keep);
             }
-            total += step_sum;
+#pragma unroll
+            for (int c = 0; c < kCols / 2; c += 16) {
+                tmem_st16(tp + c, reinterpret_cast<const uint32_t(&)[16]>(hp[c]));
+                if constexpr (kSplit) tmem_st16(tp + St::kLo + c, reinterpret_cast<const uint32_t(&)[16]>(lp[kSplit ? c : 0]));
+            }
             tmem_st_wait();
             tc_fence_before();
             __syncwarp();
@@ -587,7 +574,9 @@ __global__ void __launch_bounds__(Step<T>::kThreads, 1) attention_prompt_kernel(
 #pragma unroll
                         for (int k = 0; k < 4; k++) mma_f16_ss(ts, q + 2 * k, b + 2 * k, idesc_s, qp + kp + k > 0);
                     }
+                // the products' end, and (by a plain arrive) the converters' scales of the step, which this warp has seen
                 mma_commit_elect(&s.s_full[t]);
+                if (lane == 0) mbar_arrive(&s.s_full[t]);
             };
             scores(0);
             for (int i = 0; i < steps && ok; i++) {
