@@ -3,11 +3,11 @@
 // A row's query heads that share a kv head (at most 16 at a time) attend
 // together; such an item reads one 8704-byte record per page.  All records of
 // a call, item after item, are dealt out evenly: worker w of W (a warp) takes
-// records [T w / W, T (w + 1) / W), whatever the rows' lengths are, so one
+// its share in order, T / W of them or one more, whatever the rows' lengths are, so one
 // long row fills the card as well as many ragged ones.  A worker streams its
-// records through its own ring in shared memory (one bulk copy each, 8 warps
-// x 3 records = 209 KB in flight an SM against the ~45 KB that bandwidth times
-// latency asks for) and keeps a running maximum, sum and output per head:
+// records through its own ring in shared memory (one bulk copy each, 12 warps
+// x 2 records = 209 KB in flight an SM against the ~45 KB that bandwidth times
+// latency asks for; 8 warps x 3 took 239 us where these take 222) and keeps a running maximum, sum and output per head:
 //   S = Q K^T, O += (e vs) V   mma.sync m16n8k16 (heads x positions / dims);
 // the codes become fp16 exactly in registers, from the fragments the pages
 // hold.  Tensor cores because a position costs 128 products a head and 128
@@ -28,7 +28,7 @@ namespace ndl {
 
 namespace {
 
-constexpr int kSplitWarps = 8, kSplitThreads = 32 * kSplitWarps, kSplitStages = 3;
+constexpr int kSplitWarps = 12, kSplitThreads = 32 * kSplitWarps, kSplitStages = 2;
 constexpr int kSplitCtas = 148;                       // one CTA an SM
 constexpr int kSplitWorkers = kSplitCtas * kSplitWarps;
 constexpr int kHeadBlock = 16;                        // query heads an item holds
@@ -36,6 +36,7 @@ constexpr uint32_t kSplitWait = 1u << 22;             // tests of about a micros
 // A piece: per head 64 outputs, m and l (padded to 16 bytes).
 constexpr int kPieceHead = 68;
 constexpr int kJoinThreads = 256;
+constexpr int kJoinItems = 592;                       // items from which a CTA joins all heads of one
 
 struct SplitArgs {
     const void *q;
@@ -60,12 +61,25 @@ __device__ __forceinline__ bool row_pages(const SplitArgs &a, int row, int &firs
     last = (len - 1) / kPagePositions + 1;
     return true;
 }
-__device__ __forceinline__ int worker_count(long long records) {
-    return records < kSplitWorkers ? (int)records : kSplitWorkers;
+// 64-bit quotients are slow, and records hardly ever need them.
+__device__ __forceinline__ long long quotient(long long a, int b) {
+    return a >> 32 == 0 ? (long long)((uint32_t)a / (uint32_t)b) : a / b;
 }
-__device__ __forceinline__ long long worker_start(long long records, int workers, int w) {
-    return records * w / workers;
-}
+// The records' shares: workers 0 .. more - 1 take each + 1, the others each.
+struct Shares {
+    long long each;
+    int workers, more;
+    __device__ __forceinline__ explicit Shares(long long records) {
+        workers = records < kSplitWorkers ? (int)records : kSplitWorkers;
+        each = workers ? quotient(records, workers) : 0;
+        more = (int)(records - each * workers);
+    }
+    __device__ __forceinline__ long long start(int w) const { return each * w + min(w, more); }
+    __device__ __forceinline__ int holder(long long record) const {
+        const long long split = (each + 1) * more;
+        return record < split ? (int)quotient(record, (int)(each + 1)) : more + (int)quotient(record - split, (int)each);
+    }
+};
 
 struct SplitSmem {
     uint8_t ring[kSplitWarps][kSplitStages][kKvBlockBytes];
@@ -317,71 +331,90 @@ __global__ void __launch_bounds__(kSplitThreads, 1) attention_split_kernel(Split
     const int virtual_heads = a.c.heads * a.blocks;
     pdl_trigger();  // the joining kernel waits for this one's end by itself
 
-    // Records before each row: a thread sums a run of rows, the CTA scans the runs.
-    const int run = (a.rows + kSplitThreads - 1) / kSplitThreads;
-    {
-        long long mine = 0;
-        for (int i = threadIdx.x * run; i < min(a.rows, (int)(threadIdx.x + 1) * run); i++) {
-            int first, last;
-            row_pages(a, i, first, last);
-            mine += (long long)(last - first) * virtual_heads;
-        }
-        long long sum = mine;
+    for (int i = lane; i < kSplitStages; i += 32) mbar_init(&s.full[warp][i], 1);
+    fence_mbar_init();
+    __syncwarp();
+    // Records before each row.  Up to 32 rows: every warp scans them by itself, lane = row.  More: a thread sums a run
+    // of rows, the CTA scans the runs.
+    const int worker = warp * gridDim.x + blockIdx.x;  // the first workers sit on different SMs
+    const auto row_records = [&](int row) {
+        int first, last;
+        row_pages(a, row, first, last);
+        return (long long)(last - first) * virtual_heads;
+    };
+    const auto scan = [&](long long x) {  // over the warp, this lane included
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const long long up = __shfl_up_sync(0xffffffffu, sum, o);
-            if (lane >= o) sum += up;
+            const long long up = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += up;
         }
+        return x;
+    };
+    SplitCursor cur;
+    long long records, at;  // at: records before the first one's row
+    const bool few = a.rows <= 32;
+    const int run = (a.rows + kSplitThreads - 1) / kSplitThreads;
+    if (few) {
+        const long long mine = lane < a.rows ? row_records(lane) : 0, upto = scan(mine);
+        records = __shfl_sync(0xffffffffu, upto, 31);
+        if (blockIdx.x == 0 && warp == 0 && lane <= a.rows) {
+            a.prefix[lane] = upto - mine;
+            if (lane == 31) a.prefix[a.rows] = upto;  // 32 rows: one entry more than lanes
+        }
+        const Shares shares(records);
+        if (worker >= shares.workers) return;
+        const long long begin = shares.start(worker);
+        const int l = __ffs(__ballot_sync(0xffffffffu, upto > begin)) - 1;
+        cur.row = l;
+        at = __shfl_sync(0xffffffffu, upto - mine, l);
+    } else {
+        long long mine = 0;
+        for (int i = threadIdx.x * run; i < min(a.rows, (int)(threadIdx.x + 1) * run); i++) mine += row_records(i);
+        const long long sum = scan(mine);
         if (lane == 31) s.sums[warp + 1] = sum;
-        if (threadIdx.x < kSplitWarps * kSplitStages) mbar_init(&s.full[0][0] + threadIdx.x, 1);
-        fence_mbar_init();
         __syncthreads();
-        long long before = 0;
+        long long before = sum;
         for (int w = 0; w < warp; w++) before += s.sums[w + 1];
         __syncthreads();
-        s.sums[threadIdx.x + 1] = before + sum;
+        s.sums[threadIdx.x + 1] = before;
         if (threadIdx.x == 0) s.sums[0] = 0;
         __syncthreads();
         if (blockIdx.x == 0) {
-            long long at = before + sum - mine;
+            long long x = before - mine;
             for (int i = threadIdx.x * run; i < min(a.rows, (int)(threadIdx.x + 1) * run); i++) {
-                int first, last;
-                row_pages(a, i, first, last);
-                a.prefix[i] = at;
-                at += (long long)(last - first) * virtual_heads;
+                a.prefix[i] = x;
+                x += row_records(i);
             }
             if (threadIdx.x == 0) a.prefix[a.rows] = s.sums[kSplitThreads];
         }
-    }
-    const long long records = s.sums[kSplitThreads];
-    const int workers = worker_count(records);
-    const int worker = warp * gridDim.x + blockIdx.x;  // the first workers sit on different SMs
-    if (worker >= workers) return;
-    const long long begin = worker_start(records, workers, worker), end = worker_start(records, workers, worker + 1);
-
-    // the first record's row, item and page
-    SplitCursor cur;
-    long long item_at;  // record index of the current item's first page
-    {
+        records = s.sums[kSplitThreads];
+        const Shares shares(records);
+        if (worker >= shares.workers) return;
+        const long long begin = shares.start(worker);
         int lo = 0, hi = kSplitThreads;  // the run: sums[lo] <= begin < sums[hi]
         while (hi - lo > 1) {
             const int mid = (lo + hi) >> 1;
             if (s.sums[mid] <= begin) lo = mid;
             else hi = mid;
         }
-        long long at = s.sums[lo];
-        int row = lo * run;
-        for (;; row++) {
-            row_pages(a, row, cur.first, cur.last);
-            const long long n = (long long)(cur.last - cur.first) * virtual_heads;
+        at = s.sums[lo];
+        for (cur.row = lo * run;; cur.row++) {
+            const long long n = row_records(cur.row);
             if (begin < at + n) break;
             at += n;
         }
+    }
+    const Shares shares(records);
+    const long long begin = shares.start(worker), end = shares.start(worker + 1);
+
+    // the first record's item and page
+    row_pages(a, cur.row, cur.first, cur.last);
+    long long item_at;  // record index of the current item's first page
+    {
         const int pages = cur.last - cur.first;
-        cur.row = row;
-        cur.item = (int)((begin - at) / pages);
-        cur.page = cur.first + (int)((begin - at) % pages);
+        cur.item = (int)quotient(begin - at, pages);
         item_at = at + (long long)cur.item * pages;
+        cur.page = cur.first + (int)(begin - item_at);
     }
     // the copies' own place, ahead of the reading
     SplitCursor ahead = cur;
@@ -501,22 +534,29 @@ __global__ void __launch_bounds__(kSplitThreads, 1) attention_split_kernel(Split
     }
 }
 
-// Joins the pieces of one item (CTA) in worker order:
-//   out = sum w_i o_i / sum w_i,  w_i = l_i 2^(m_i - max m)
-// and writes the rows that have no records.
+// Joins the pieces of an item in worker order,
+//   out = sum w_i o_i / sum w_i,  w_i = l_i 2^(m_i - max m),
+// and writes the rows that have no records.  A CTA takes an item's heads, or
+// with `split_heads` one of them; its warps share out the heads, and what is
+// left of them the pieces of a head, whose loads go out in batches.
 template <class T>
-__global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(SplitArgs a) {
-    __shared__ float acc[kJoinThreads / 32][kHeadDim], weight[kJoinThreads / 32], tops[kJoinThreads / 32];
+__global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(SplitArgs a, int split_heads) {
+    constexpr int kWarps = kJoinThreads / 32, kBatch = 8;
+    __shared__ float acc[kWarps][kHeadDim];
+    __shared__ float2 part_ml[kWarps];
     pdl_wait();
     const int virtual_heads = a.c.heads * a.blocks;
-    const int row = blockIdx.x / virtual_heads, item = blockIdx.x - row * virtual_heads;
+    const int unit = split_heads ? blockIdx.x / a.piece_heads : blockIdx.x;
+    const int row = unit / virtual_heads, item = unit - row * virtual_heads;
     const int kv = item / a.blocks, block = item - kv * a.blocks;
-    const int heads = min(kHeadBlock, a.group - block * kHeadBlock);
+    const int first_head = split_heads ? blockIdx.x - unit * a.piece_heads : 0;
+    const int heads = min(split_heads ? 1 : kHeadBlock, a.group - block * kHeadBlock - first_head);
+    if (heads <= 0) return;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     T *out = static_cast<T *>(a.out) + (size_t)row * a.out_stride +
-             ((size_t)kv * a.group + block * kHeadBlock) * kHeadDim;
+             ((size_t)kv * a.group + block * kHeadBlock + first_head) * kHeadDim;
     const long long before = a.prefix[row], records = a.prefix[a.rows];
-    const long long pages = (a.prefix[row + 1] - before) / virtual_heads;
+    const long long pages = quotient(a.prefix[row + 1] - before, virtual_heads);
     if (pages == 0) {
         int first, last;
         const bool good = row_pages(a, row, first, last);
@@ -525,48 +565,61 @@ __global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(SplitArgs 
             out[i] = from_float<T>(good ? 0.0f : __int_as_float(0x7fc00000));
         return;
     }
-    const int workers = worker_count(records);
+    const Shares shares(records);
     const long long begin = before + item * pages, end = begin + pages;
     // the workers whose ranges hold its first and last record
-    auto holder = [&](long long rec) {
-        int w = (int)(((double)rec + 0.5) * workers / (double)records);
-        w = max(0, min(workers - 1, w));
-        while (worker_start(records, workers, w) > rec) w--;
-        while (worker_start(records, workers, w + 1) <= rec) w++;
-        return w;
-    };
-    const int w0 = holder(begin), w1 = holder(end - 1);
+    const int w0 = shares.holder(begin), w1 = shares.holder(end - 1);
     if (w0 == w1) return;  // that worker wrote it
-    const int first_piece = worker_start(records, workers, w0) == begin ? 0 : 1;
-    for (int h = 0; h < heads; h++) {
+    const int first_piece = shares.start(w0) == begin ? 0 : 1;
+    const int parts = heads >= kWarps ? 1 : kWarps / heads;       // warps a head
+    const int count = w1 - w0 + 1, per = (count + parts - 1) / parts;
+    const int part = warp % parts, from = w0 + part * per, to = min(w1 + 1, from + per);
+    for (int h0 = 0; h0 < heads; h0 += kWarps / parts) {
+        const int h = h0 + warp / parts;
         float top = -INFINITY, sum = 0.0f, o0 = 0.0f, o1 = 0.0f;
-        // a warp takes a run of the pieces, in order
-        const int count = w1 - w0 + 1, per = (count + kJoinThreads / 32 - 1) / (kJoinThreads / 32);
-        const int from = w0 + warp * per, to = min(w1 + 1, from + per);
-#pragma unroll 4
-        for (int w = from; w < to; w++) {
-            const float *p = a.pieces + (((size_t)w * 2 + (w == w0 ? first_piece : 0)) * a.piece_heads + h) * kPieceHead;
-            const float2 ml = *reinterpret_cast<const float2 *>(p + kHeadDim);
-            const float2 v = *reinterpret_cast<const float2 *>(p + 2 * lane);
-            const float m = fmaxf(top, ml.x);
-            const float keep = top == m ? 1.0f : exp2f(top - m), add = ml.x == m ? ml.y : ml.y * exp2f(ml.x - m);
-            sum = sum * keep + add, o0 = o0 * keep + add * v.x, o1 = o1 * keep + add * v.y;
-            top = m;
-        }
-        acc[warp][2 * lane] = o0, acc[warp][2 * lane + 1] = o1;
-        if (lane == 0) weight[warp] = sum, tops[warp] = top;
-        __syncthreads();
-        if (threadIdx.x < kHeadDim) {
-            float m = -INFINITY, w = 0.0f, o = 0.0f;
-            for (int i = 0; i < kJoinThreads / 32; i++) m = fmaxf(m, tops[i]);
-            for (int i = 0; i < kJoinThreads / 32; i++) {
-                if (tops[i] == -INFINITY && weight[i] == 0.0f) continue;  // no pieces
-                const float f = tops[i] == m ? 1.0f : exp2f(tops[i] - m);
-                w += weight[i] * f, o += acc[i][threadIdx.x] * f;
+        if (h < heads) {
+            const auto piece = [&](int w) {
+                return a.pieces + (((size_t)w * 2 + (w == w0 ? first_piece : 0)) * a.piece_heads + first_head + h) * kPieceHead;
+            };
+            for (int base = from; base < to; base += kBatch) {
+                float2 ml[kBatch], v[kBatch];
+#pragma unroll
+                for (int j = 0; j < kBatch; j++) {
+                    const bool there = base + j < to;
+                    const float *p = piece(there ? base + j : from);
+                    ml[j] = there ? *reinterpret_cast<const float2 *>(p + kHeadDim) : make_float2(-INFINITY, 0.0f);
+                    v[j] = *reinterpret_cast<const float2 *>(p + 2 * lane);
+                }
+                float m = top;
+#pragma unroll
+                for (int j = 0; j < kBatch; j++) m = fmaxf(m, ml[j].x);
+                const float keep = top == m ? 1.0f : exp2f(top - m);
+                sum *= keep, o0 *= keep, o1 *= keep;
+                top = m;
+#pragma unroll
+                for (int j = 0; j < kBatch; j++) {
+                    if (base + j >= to) break;
+                    const float f = ml[j].x == m ? ml[j].y : ml[j].y * exp2f(ml[j].x - m);
+                    sum += f, o0 = fmaf(f, v[j].x, o0), o1 = fmaf(f, v[j].y, o1);
+                }
             }
-            out[h * kHeadDim + threadIdx.x] = from_float<T>(o / w);
         }
-        __syncthreads();
+        if (parts > 1) {  // the warps of a head, in order (heads < kWarps: one round)
+            acc[warp][2 * lane] = o0, acc[warp][2 * lane + 1] = o1;
+            if (lane == 0) part_ml[warp] = make_float2(top, sum);
+            __syncthreads();
+            if (part != 0 || h >= heads) return;
+            float m = -INFINITY;
+            for (int i = 0; i < parts; i++) m = fmaxf(m, part_ml[warp + i].x);
+            sum = o0 = o1 = 0.0f;
+            for (int i = 0; i < parts; i++) {
+                const float2 ml = part_ml[warp + i];
+                if (w0 + i * per > w1) continue;  // no pieces
+                const float f = ml.x == m ? 1.0f : exp2f(ml.x - m);
+                sum += ml.y * f, o0 += acc[warp + i][2 * lane] * f, o1 += acc[warp + i][2 * lane + 1] * f;
+            }
+        }
+        if (h < heads) store2(out + h * kHeadDim + 2 * lane, o0 / sum, o1 / sum);
     }
 }
 
@@ -636,8 +689,11 @@ extern "C" NDL_API int ndl_attention_split(const void *q, long long q_stride, in
         const int rc2 = check_launch("attention_split");
         if (rc2 != NDL_OK) return rc2;
         PdlScope early(true);  // the join's launch overlaps the kernel above; it waits for its end before reading
-        launch_kernel(attention_join_kernel<T>, dim3((unsigned)(rows * kv_heads * a.blocks)), dim3(kJoinThreads), 0,
-                      (cudaStream_t)stream, a);
+        // few items may have many pieces each: a CTA a head then
+        const long long items = (long long)rows * kv_heads * a.blocks;
+        const int split_heads = items < kJoinItems;
+        launch_kernel(attention_join_kernel<T>, dim3((unsigned)(items * (split_heads ? a.piece_heads : 1))),
+                      dim3(kJoinThreads), 0, (cudaStream_t)stream, a, split_heads);
         return check_launch("attention_join");
     });
 }
