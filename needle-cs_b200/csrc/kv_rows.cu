@@ -7,13 +7,12 @@
 // the same 64 values.  Gather: code * scale, the values the pages stand for.
 //
 // Both are bound by memory, and by how the pages scatter a row: its 64 value
-// bytes lie 64 bytes apart, its keys in 16 words.  So rows of a block that
-// follow one another inside a 16-position chunk of a page (a run) go to one
-// warp a head: a lane holds 32 dims of one position; keys change hands between
-// positions 8 apart and move as 16-byte chunks, values turn around in shared
-// memory (4x4 bytes by permutes) and move 4 positions of a dim at a time.
-// Other rows, as a decode step has them, go 16 to a warp, each by its words
-// and bytes.
+// bytes lie 64 bytes apart, its keys in 16 words.  So a warp takes up to 16
+// rows of a head, eight lanes a row where rows are read or written (four rows
+// an access), and turns their codes around in shared memory.  Rows that follow
+// one another inside a 16-position chunk of a page (a run) then move their keys
+// as 16-byte chunks and their values 4 positions of a dim at a time (4x4 bytes
+// by permutes); others, as a decode step has them, go by words and bytes.
 #include "paged.cuh"
 
 namespace ndl {
@@ -49,51 +48,84 @@ struct KvRowsArgs {
 };
 
 constexpr int kRowWarps = 2, kRowThreads = 32 * kRowWarps;
-constexpr int kBlockRows = 32;           // rows of a block, at most: a warp looks them over
+constexpr int kBlockRows = 32;           // rows of a block, at most
 constexpr int kChunk = 16;               // positions of a chunk: 16 bytes of a value dim
+constexpr int kSeenRows = kBlockRows + kChunk;  // and of the runs that start in it: a run is the block's it starts in
 constexpr int kShortRun = 3;             // rows from which a run is worth a warp
 constexpr int kTurnRow = kHeadDim + 4;   // a position's codes in shared memory: 17 words, so positions on different banks
 
 struct KvRowsSmem {
     __align__(16) uint8_t turn[kRowWarps][kChunk * kTurnRow];
-    uint8_t *rec[kBlockRows];  // the row's record of head 0, null for a padding or bad row
-    int place[kBlockRows];     // its position in the page
-    int bad[kBlockRows];
-    int runs[kBlockRows], singles[kBlockRows];  // runs: first row | length << 8
+    uint8_t *rec[kSeenRows];  // the row's record of head 0, null for a padding or bad row
+    int place[kSeenRows];     // its position in the page
+    int bad[kSeenRows];
+    int runs[kBlockRows], singles[kSeenRows];  // runs: first row | length << 8
     int run_count, single_count;
 };
 
 // The block's rows: where they go, its runs and its single rows.
 __device__ __forceinline__ void kv_rows_block(const KvRowsArgs &a, KvRowsSmem &s, int first) {
     if (threadIdx.x < 32) {
-        const int n = min(a.block_rows, a.rows - first), i = threadIdx.x;
-        uint8_t *rec = nullptr;
-        int place = 0, bad = 0;
-        if (i < n) {
+        const int lane = threadIdx.x;
+        const int own = min(a.block_rows, a.rows - first), n = min(own + kChunk, a.rows - first);
+        uint8_t *rec[2] = {nullptr, nullptr};
+        int place[2] = {0, 0};
+        uint64_t starts = 0;
+        // the row before the block and, behind, the rows its last run may reach
+        const auto look = [&](int i, uint8_t *&rec, int &place, bool keep) {
             const int pos = a.row_pos[first + i], slot = a.row_slot[first + i];
+            int bad = 0;
             if (pos >= 0) {
                 const int page = slot >= 0 && slot < a.c.slots ? cache_page(a.c, slot, pos / kPagePositions) : -1;
                 bad = page < 0;
                 place = pos % kPagePositions;
                 if (!bad) rec = cache_record(a.c, page, 0);
-                else if (a.c.status) atomicOr(a.c.status, kStatusBadPage);
+                else if (keep && i < own && a.c.status) atomicOr(a.c.status, kStatusBadPage);
             }
-            s.rec[i] = rec, s.place[i] = place, s.bad[i] = bad;
+            if (keep) s.rec[i] = rec, s.place[i] = place, s.bad[i] = bad;
+        };
+        uint8_t *before = nullptr;
+        int before_place = 0;
+        if (lane == 0 && first > 0) look(-1, before, before_place, false);
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+            if (lane + 32 * h < n) look(lane + 32 * h, rec[h], place[h], true);
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const int i = lane + 32 * h;
+            unsigned long long up = __shfl_up_sync(0xffffffffu, (unsigned long long)rec[h], 1);
+            int up_place = __shfl_up_sync(0xffffffffu, place[h], 1);
+            if (lane == 0) up = (unsigned long long)before, up_place = before_place;
+            before = (uint8_t *)__shfl_sync(0xffffffffu, (unsigned long long)rec[h], 31);
+            before_place = __shfl_sync(0xffffffffu, place[h], 31);
+            const bool start = i < n && !(rec[h] && (unsigned long long)rec[h] == up && place[h] == up_place + 1 &&
+                                          (place[h] & (kChunk - 1)) != 0);
+            starts |= (uint64_t)__ballot_sync(0xffffffffu, start) << (32 * h);
         }
-        const unsigned long long before = __shfl_up_sync(0xffffffffu, (unsigned long long)rec, 1);
-        const int before_place = __shfl_up_sync(0xffffffffu, place, 1);
-        const bool starts = i < n && !(i > 0 && rec && (unsigned long long)rec == before && place == before_place + 1 &&
-                                       (place & (kChunk - 1)) != 0);
-        const unsigned mask = __ballot_sync(0xffffffffu, starts);
-        const unsigned upto = mask & (0xFFFFFFFFu >> (31 - i)), behind = i < 31 ? mask >> (i + 1) : 0;
-        const int start = 31 - __clz((int)upto), end = behind ? i + __ffs((int)behind) : n;
-        const bool in_run = i < n && rec && end - start >= kShortRun;
-        const unsigned runs = __ballot_sync(0xffffffffu, starts && in_run);
-        const unsigned singles = __ballot_sync(0xffffffffu, i < n && !in_run);
-        const unsigned below = (1u << i) - 1;
-        if (starts && in_run) s.runs[__popc(runs & below)] = i | (end - start) << 8;
-        if (i < n && !in_run) s.singles[__popc(singles & below)] = i;
-        if (i == 0) s.run_count = __popc(runs), s.single_count = __popc(singles);
+        const uint64_t owned = own >= 64 ? ~0ull : (1ull << own) - 1;  // rows of the block itself
+        uint64_t runs = 0, singles = 0;
+        int length[2];
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const int i = lane + 32 * h;
+            const uint64_t upto = starts & owned & (~0ull >> (63 - i)), behind = i < 63 ? starts >> (i + 1) : 0;
+            const int start = 63 - __clzll((long long)upto);  // -1: the run of an earlier block
+            const int end = behind ? i + __ffsll((long long)behind) : n;
+            // behind the block only rows of a run that starts in it
+            const bool ours = i < n && start >= 0 && (i < own || !(starts >> own & (~0ull >> (63 - i + own))));
+            length[h] = end - i;
+            const bool in_run = ours && rec[h] && end - start >= kShortRun;
+            runs |= (uint64_t)__ballot_sync(0xffffffffu, in_run && start == i) << (32 * h);
+            singles |= (uint64_t)__ballot_sync(0xffffffffu, ours && !in_run) << (32 * h);
+        }
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const int i = lane + 32 * h;
+            const uint64_t below = (1ull << i) - 1;
+            if (runs >> i & 1) s.runs[__popcll(runs & below)] = i | length[h] << 8;
+            if (singles >> i & 1) s.singles[__popcll(singles & below)] = i;
+        }
+        if (lane == 0) s.run_count = __popcll(runs), s.single_count = __popcll(singles);
     }
     __syncthreads();
 }
@@ -106,256 +138,295 @@ __device__ __forceinline__ void turn4(uint32_t (&w)[4]) {
     w[2] = __byte_perm(c, d, 0x5410), w[3] = __byte_perm(c, d, 0x7632);
 }
 
-// Lane (position r = lane & 15 of the chunk, half = lane >> 4): dims 32 half .. + 31, word c of them at w[c].  In the
-// pages, chunk (row & 7, column t) of a 32-dim step holds words (r, t), (r + 8, t), (r, t + 4), (r + 8, t + 4); the lane
-// of r < 8 moves columns 0 and 1 of both positions, that of r + 8 columns 2 and 3.
-__device__ __forceinline__ void swap_columns(uint32_t (&w)[8], bool upper) {
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const int give_low = (i >> 1) * 4 + (i & 1), give_high = give_low + 2;  // words of columns 0, 1 / 2, 3
-        const uint32_t got = __shfl_xor_sync(0xffffffffu, upper ? w[give_low] : w[give_high], 8);
-        if (upper) w[give_low] = got;
-        else w[give_high] = got;
-    }
-}
-
+// Eight lanes a row: lane -> dims 8 (lane & 7) .. of row 4 j + (lane >> 3).
 template <class T>
-__device__ __forceinline__ void load32(const T *p, float (&x)[32]) {
-    if constexpr (sizeof(T) == 4) {
+struct Eight {
+    uint4 raw[sizeof(T) == 4 ? 2 : 1];
+    __device__ __forceinline__ void load(const T *p) {
 #pragma unroll
-        for (int i = 0; i < 32; i += 4) {
-            const float4 v = *reinterpret_cast<const float4 *>(p + i);
-            x[i] = v.x, x[i + 1] = v.y, x[i + 2] = v.z, x[i + 3] = v.w;
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 32; i += 8) {
-            const uint4 v = *reinterpret_cast<const uint4 *>(p + i);
-            const T *h = reinterpret_cast<const T *>(&v);
-#pragma unroll
-            for (int j = 0; j < 8; j++) x[i + j] = to_float(h[j]);
-        }
+        for (int i = 0; i < (int)(sizeof(T) / 2); i++) raw[i] = *(reinterpret_cast<const uint4 *>(p) + i);
     }
-}
-template <class T>
-__device__ __forceinline__ void store32(T *p, const float (&x)[32]) {
-    if constexpr (sizeof(T) == 4) {
+    __device__ __forceinline__ float get(int i) const { return to_float(reinterpret_cast<const T *>(raw)[i]); }
+    __device__ __forceinline__ void set(int i, float x) { reinterpret_cast<T *>(raw)[i] = from_float<T>(x); }
+    __device__ __forceinline__ void store(T *p) const {
 #pragma unroll
-        for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4 *>(p + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 32; i += 8) {
-            alignas(16) T h[8];
-#pragma unroll
-            for (int j = 0; j < 8; j++) h[j] = from_float<T>(x[i + j]);
-            *reinterpret_cast<uint4 *>(p + i) = *reinterpret_cast<const uint4 *>(h);
-        }
+        for (int i = 0; i < (int)(sizeof(T) / 2); i++) *(reinterpret_cast<uint4 *>(p) + i) = raw[i];
     }
-}
-
-// The codes of a lane's 32 dims and its position's scale (the partner holds the other 32).  Adding 1.5 * 2^23 rounds to
-// an integer, ties to even, and leaves it in the low byte; a NaN becomes -128 as the quantizer's clamp makes it.
-__device__ __forceinline__ float quantize32(const float (&x)[32], uint32_t (&w)[8]) {
-    float peak = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 32; i++) peak = fmaxf(peak, fabsf(x[i]));
-    peak = fmaxf(peak, __shfl_xor_sync(0xffffffffu, peak, 16));
-    const float scale = peak > 0.0f ? __fdiv_rn(peak, 127.0f) : 1.0f;
-    const float inverse = __fdiv_rn(1.0f, scale);
-#pragma unroll
-    for (int c = 0; c < 8; c++) {
-        uint32_t b[4];
-#pragma unroll
-        for (int j = 0; j < 4; j++)
-            b[j] = __float_as_uint(__fadd_rn(fminf(fmaxf(__fmul_rn(x[4 * c + j], inverse), -128.0f), 127.0f), 12582912.0f));
-        w[c] = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
-    }
-    return scale;
-}
-
-// A warp's share of a block: run i of the block, then 16 single rows a task.
-struct KvTask {
-    int row;              // this lane's row of the block
-    bool mine;            // it has one
-    uint8_t *rec;         // its record (null: padding or bad)
-    int place;            // its position in the page
-    bool run;             // the warp's rows are a run,
-    int from, to, chunk;  // positions from .. to - 1 of a 16-position chunk
 };
-__device__ __forceinline__ KvTask kv_task(const KvRowsSmem &s, int i, int head, int r) {
-    KvTask t;
-    t.run = i < s.run_count;
-    if (t.run) {
-        const int row0 = s.runs[i] & 0xFF, n = s.runs[i] >> 8, place = s.place[row0];
-        t.from = place & (kChunk - 1), t.to = t.from + n, t.chunk = place >> 4;
-        t.mine = r >= t.from && r < t.to;
-        t.row = row0 + (t.mine ? r - t.from : 0);
-        t.rec = s.rec[row0] + (size_t)head * kKvBlockBytes;
-        t.place = t.chunk * kChunk + r;
-    } else {
-        const int j = (i - s.run_count) * kChunk + r;
-        t.mine = j < s.single_count;
-        t.row = s.singles[t.mine ? j : 0];
-        t.rec = s.rec[t.row];
-        if (t.rec) t.rec += (size_t)head * kKvBlockBytes;
-        t.place = s.place[t.row];
-        t.from = t.to = t.chunk = 0;
+
+// Scales and inverses of four rows, of which the lane holds eight dims each.  The two quotients of a row are one lane's.
+template <class T>
+__device__ __forceinline__ void row_scales(const Eight<T> (&x)[4], int lane, float (&scale)[4], float (&inverse)[4]) {
+    float peak[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        peak[j] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; i++) peak[j] = fmaxf(peak[j], fabsf(x[j].get(i)));
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) peak[j] = fmaxf(peak[j], __shfl_xor_sync(0xffffffffu, peak[j], o));
     }
-    return t;
+    const float p01 = lane & 1 ? peak[1] : peak[0], p23 = lane & 1 ? peak[3] : peak[2], mine = lane & 2 ? p23 : p01;
+    const float s = mine > 0.0f ? __fdiv_rn(mine, 127.0f) : 1.0f;
+    const float v = __fdiv_rn(1.0f, s);
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        scale[j] = __shfl_sync(0xffffffffu, s, (lane & 24) | j);
+        inverse[j] = __shfl_sync(0xffffffffu, v, (lane & 24) | j);
+    }
 }
+// Eight codes.  Adding 1.5 * 2^23 rounds to an integer, ties to even, and leaves it in the low byte; a NaN becomes -128
+// as the quantizer's clamp makes it.
+template <class T>
+__device__ __forceinline__ uint2 quantize8(const Eight<T> &x, float inverse) {
+    uint32_t b[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+        b[i] = __float_as_uint(__fadd_rn(fminf(fmaxf(__fmul_rn(x.get(i), inverse), -128.0f), 127.0f), 12582912.0f));
+    return make_uint2(__byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410),
+                      __byte_perm(__byte_perm(b[4], b[5], 0x0040), __byte_perm(b[6], b[7], 0x0040), 0x5410));
+}
+// Eight codes times a scale (the code by the low mantissa byte of 2^23, less 2^23 + 128).
+template <class T>
+__device__ __forceinline__ void scale8(uint2 w, float scale, Eight<T> &x) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const uint32_t u = (i < 4 ? w.x : w.y) ^ 0x80808080u;
+        x.set(i, __fmul_rn(__uint_as_float(__byte_perm(u, 0x4B000000u, 0x7440 + (i & 3))) - 8388736.0f, scale));
+    }
+}
+
+// A warp's share of a block: run i of the block, then 16 single rows a task.  Its 16 places: the positions of the run's
+// chunk, or one a single row.
+struct KvTask {
+    bool run;
+    int from, to;  // places that have a row
+    int row0;      // run: row of place `from`; else number of the first single row
+    uint8_t *rec;  // run: its record
+    int chunk;     // run: its chunk of the page
+};
 __device__ __forceinline__ int kv_tasks(const KvRowsSmem &s) {
     return s.run_count + (s.single_count + kChunk - 1) / kChunk;
 }
+__device__ __forceinline__ KvTask kv_task(const KvRowsSmem &s, int i, int head) {
+    KvTask t;
+    t.run = i < s.run_count;
+    if (t.run) {
+        t.row0 = s.runs[i] & 0xFF;
+        const int place = s.place[t.row0];
+        t.from = place & (kChunk - 1), t.to = t.from + (s.runs[i] >> 8), t.chunk = place >> 4;
+        t.rec = s.rec[t.row0] + (size_t)head * kKvBlockBytes;
+    } else {
+        t.row0 = (i - s.run_count) * kChunk;
+        t.from = 0, t.to = min(kChunk, s.single_count - t.row0);
+        t.rec = nullptr, t.chunk = 0;
+    }
+    return t;
+}
+// The block's row at a place that has one.
+__device__ __forceinline__ int kv_row(const KvRowsSmem &s, const KvTask &t, int p) {
+    return t.run ? t.row0 + p - t.from : s.singles[t.row0 + p];
+}
 
 template <class T>
-__global__ void __launch_bounds__(kRowThreads, 12) kv_append_kernel(KvRowsArgs a) {
+__global__ void __launch_bounds__(kRowThreads, 10) kv_append_kernel(KvRowsArgs a) {
     __shared__ KvRowsSmem s;
     const int first = blockIdx.x * a.block_rows, head = blockIdx.y;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane & 15, half = lane >> 4;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     kv_rows_block(a, s, first);
     const int tasks = kv_tasks(s);
+    uint32_t *turn = reinterpret_cast<uint32_t *>(s.turn[warp]);
+    constexpr int kRow = kTurnRow / 4;
     for (int i = warp; i < tasks; i += kRowWarps) {
-        const KvTask t = kv_task(s, i, head, r);
-        const size_t at = first + t.row;
-        float x[32];
-        uint32_t w[8];
-        load32(static_cast<const T *>(a.k) + at * a.k_stride + head * kHeadDim + 32 * half, x);
-        const float ks = quantize32(x, w);
-        load32(static_cast<const T *>(a.v) + at * a.v_stride + head * kHeadDim + 32 * half, x);
-        const bool writes = t.mine && t.rec;
-        if (writes && half == 0) reinterpret_cast<float *>(t.rec + kKScaleOffset)[k_scale_index(t.place)] = ks;
-        if (t.run) {
-            const bool partner = (r ^ 8) >= t.from && (r ^ 8) < t.to;
-            swap_columns(w, r >= 8);
-            // words (position, column) and (position + 8, column) of columns t0 and t0 + 1
-            const int t0 = r >= 8 ? 2 : 0;
-            const bool low = r >= 8 ? partner : t.mine, high = r >= 8 ? t.mine : partner;
+        const KvTask t = kv_task(s, i, head);
+        Eight<T> x[2][4];
 #pragma unroll
-            for (int j = 0; j < 2; j++) {
-                uint32_t *dst = reinterpret_cast<uint32_t *>(t.rec + t.chunk * 1024 + half * 512 + ((r & 7) * 4 + t0 + j) * 16);
-                // own words of the column, and the partner's in the place of those given away
-                const uint32_t o0 = r >= 8 ? w[2 + j] : w[j], o1 = r >= 8 ? w[6 + j] : w[4 + j];
-                const uint32_t p0 = r >= 8 ? w[j] : w[2 + j], p1 = r >= 8 ? w[4 + j] : w[6 + j];
-                const uint32_t a0 = r >= 8 ? p0 : o0, a1 = r >= 8 ? p1 : o1, b0 = r >= 8 ? o0 : p0, b1 = r >= 8 ? o1 : p1;
-                if (low && high) {
-                    *reinterpret_cast<uint4 *>(dst) = make_uint4(a0, b0, a1, b1);
-                } else {
-                    if (low) dst[0] = a0, dst[2] = a1;
-                    if (high) dst[1] = b0, dst[3] = b1;
-                }
-            }
-        } else if (writes) {
-#pragma unroll
-            for (int c = 0; c < 8; c++) *reinterpret_cast<uint32_t *>(t.rec + k_byte(t.place, 32 * half + 4 * c)) = w[c];
+        for (int j = 0; j < 4; j++) {
+            const int p = 4 * j + (lane >> 3);
+            const size_t at = first + kv_row(s, t, min(max(p, t.from), t.to - 1));
+            x[0][j].load(static_cast<const T *>(a.k) + at * a.k_stride + head * kHeadDim + (lane & 7) * 8);
+            x[1][j].load(static_cast<const T *>(a.v) + at * a.v_stride + head * kHeadDim + (lane & 7) * 8);
         }
-        const float vs = quantize32(x, w);
-        if (writes && half == 0) reinterpret_cast<float *>(t.rec + kVScaleOffset)[v_scale_index(t.place)] = vs;
-        if (t.run) {
-            uint32_t *turn = reinterpret_cast<uint32_t *>(s.turn[warp]);
+#pragma unroll
+        for (int which = 0; which < 2; which++) {
+            float scale[4], inverse[4];
+            row_scales(x[which], lane, scale, inverse);
             __syncwarp();
 #pragma unroll
-            for (int c = 0; c < 8; c++) turn[r * (kTurnRow / 4) + half * 8 + c] = w[c];
-            __syncwarp();
-            // lane -> positions 4 q .. of dims 4 c ..
-            const int q = lane & 3;
-            if (4 * q + 4 > t.from && 4 * q < t.to) {
-                const bool all = 4 * q >= t.from && 4 * q + 4 <= t.to;
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const int c = (lane >> 2) + 8 * h;
-                    uint32_t b[4];
-#pragma unroll
-                    for (int j = 0; j < 4; j++) b[j] = turn[(4 * q + j) * (kTurnRow / 4) + c];
-                    turn4(b);
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        uint8_t *dst = t.rec + v_byte(t.chunk * kChunk + 4 * q, 4 * c + j);
-                        if (all) *reinterpret_cast<uint32_t *>(dst) = b[j];
-                        else
-#pragma unroll
-                            for (int e = 0; e < 4; e++)
-                                if (4 * q + e >= t.from && 4 * q + e < t.to) dst[e] = (uint8_t)(b[j] >> (8 * e));
+            for (int j = 0; j < 4; j++) {
+                const int p = 4 * j + (lane >> 3);
+                const uint2 w = quantize8(x[which][j], inverse[j]);
+                turn[p * kRow + (lane & 7) * 2] = w.x, turn[p * kRow + (lane & 7) * 2 + 1] = w.y;
+                if (p >= t.from && p < t.to && (lane & 7) == 0) {
+                    const int row = kv_row(s, t, p), place = s.place[row];
+                    uint8_t *rec = s.rec[row];
+                    if (rec) {
+                        rec += (size_t)head * kKvBlockBytes;
+                        if (which) reinterpret_cast<float *>(rec + kVScaleOffset)[v_scale_index(place)] = scale[j];
+                        else reinterpret_cast<float *>(rec + kKScaleOffset)[k_scale_index(place)] = scale[j];
                     }
                 }
             }
-        } else if (writes) {
+            __syncwarp();
+            if (t.run && which == 0) {
+                // 16-byte chunk (32-dim step h, row & 7, column): words of positions r and r + 8, dims and dims + 16
+                const int r = lane >> 2, c = lane & 3;
+                const bool low = r >= t.from && r < t.to, high = r + 8 >= t.from && r + 8 < t.to;
 #pragma unroll
-            for (int j = 0; j < 32; j++) t.rec[v_byte(t.place, 32 * half + j)] = (uint8_t)(w[j >> 2] >> (8 * (j & 3)));
+                for (int h = 0; h < 2; h++) {
+                    uint32_t *dst = reinterpret_cast<uint32_t *>(t.rec + t.chunk * 1024 + h * 512 + lane * 16);
+                    const uint32_t *src = turn + r * kRow + h * 8 + c;
+                    const uint4 w = make_uint4(src[0], src[8 * kRow], src[4], src[8 * kRow + 4]);
+                    if (low && high) {
+                        *reinterpret_cast<uint4 *>(dst) = w;
+                    } else {
+                        if (low) dst[0] = w.x, dst[2] = w.z;
+                        if (high) dst[1] = w.y, dst[3] = w.w;
+                    }
+                }
+            } else if (t.run) {
+                // lane -> positions 4 q .. of dims 4 c ..
+                const int q = lane & 3;
+                const bool all = 4 * q >= t.from && 4 * q + 4 <= t.to;
+                if (4 * q + 4 > t.from && 4 * q < t.to) {
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        const int c = (lane >> 2) + 8 * h;
+                        uint32_t b[4];
+#pragma unroll
+                        for (int j = 0; j < 4; j++) b[j] = turn[(4 * q + j) * kRow + c];
+                        turn4(b);
+#pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            uint8_t *dst = t.rec + v_byte(t.chunk * kChunk + 4 * q, 4 * c + j);
+                            if (all) *reinterpret_cast<uint32_t *>(dst) = b[j];
+                            else
+#pragma unroll
+                                for (int e = 0; e < 4; e++)
+                                    if (4 * q + e >= t.from && 4 * q + e < t.to) dst[e] = (uint8_t)(b[j] >> (8 * e));
+                        }
+                    }
+                }
+            } else {
+                // 16 lanes a single row, two rows an access (a row's key words lie in four sectors)
+                const int c = lane & 15;
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const int p = 2 * j + (lane >> 4);
+                    if (p >= t.to) break;
+                    const int row = kv_row(s, t, p), place = s.place[row];
+                    if (!s.rec[row]) continue;
+                    uint8_t *rec = s.rec[row] + (size_t)head * kKvBlockBytes;
+                    const uint32_t w = turn[p * kRow + c];
+                    if (which == 0) *reinterpret_cast<uint32_t *>(rec + k_byte(place, 4 * c)) = w;
+                    else
+#pragma unroll
+                        for (int e = 0; e < 4; e++) rec[v_byte(place, 4 * c + e)] = (uint8_t)(w >> (8 * e));
+                }
+            }
         }
+        __syncwarp();
     }
 }
 
 template <class T>
-__global__ void __launch_bounds__(kRowThreads, 12) kv_gather_kernel(KvRowsArgs a) {
+__global__ void __launch_bounds__(kRowThreads, 10) kv_gather_kernel(KvRowsArgs a) {
     __shared__ KvRowsSmem s;
     const int first = blockIdx.x * a.block_rows, head = blockIdx.y;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane & 15, half = lane >> 4;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     kv_rows_block(a, s, first);
     const int tasks = kv_tasks(s);
+    uint32_t *turn = reinterpret_cast<uint32_t *>(s.turn[warp]);
+    constexpr int kRow = kTurnRow / 4;
     for (int i = warp; i < tasks; i += kRowWarps) {
-        const KvTask t = kv_task(s, i, head, r);
-        const size_t at = first + t.row;
-        T *k = static_cast<T *>(a.k_out) + at * a.k_stride + head * kHeadDim + 32 * half;
-        T *v = static_cast<T *>(a.v_out) + at * a.v_stride + head * kHeadDim + 32 * half;
-        uint32_t kw[8] = {}, vw[8] = {};
-        float ks = 0.0f, vs = 0.0f;
-        if (t.rec) {
-            ks = __ldg(reinterpret_cast<const float *>(t.rec + kKScaleOffset) + k_scale_index(t.place));
-            vs = __ldg(reinterpret_cast<const float *>(t.rec + kVScaleOffset) + v_scale_index(t.place));
-        } else if (s.bad[t.row]) {  // NaN; a padding row gives zeros
-            ks = vs = __int_as_float(0x7fc00000);
-        }
+        const KvTask t = kv_task(s, i, head);
+        // scales of the places this lane's eights have
+        float scale[2][4];
+        uint4 key[2], dim[2];
         if (t.run) {
-            const int t0 = r >= 8 ? 2 : 0;
-            uint4 dim[2];
-#pragma unroll
-            for (int j = 0; j < 2; j++) {
-                const uint4 c =
-                    __ldg(reinterpret_cast<const uint4 *>(t.rec + t.chunk * 1024 + half * 512 + ((r & 7) * 4 + t0 + j) * 16));
-                dim[j] = __ldg(reinterpret_cast<const uint4 *>(t.rec + v_byte(t.chunk * kChunk, lane + 32 * j)));
-                // own words of columns t0 + j in their place, the partner's in the place of what it will give
-                const uint32_t o0 = r >= 8 ? c.y : c.x, o1 = r >= 8 ? c.w : c.z, p0 = r >= 8 ? c.x : c.y, p1 = r >= 8 ? c.z : c.w;
-                kw[j] = r >= 8 ? p0 : o0, kw[4 + j] = r >= 8 ? p1 : o1;
-                kw[2 + j] = r >= 8 ? o0 : p0, kw[6 + j] = r >= 8 ? o1 : p1;
-            }
-            swap_columns(kw, r >= 8);
-            // values: dims as rows of 16 bytes, turned around to positions as rows
-            uint32_t *turn = reinterpret_cast<uint32_t *>(s.turn[warp]);
-            __syncwarp();
-#pragma unroll
-            for (int j = 0; j < 2; j++) *reinterpret_cast<uint4 *>(turn + (lane + 32 * j) * 4) = dim[j];
-            __syncwarp();
-            const int q = lane & 3;
-            uint32_t b[2][4];
 #pragma unroll
             for (int h = 0; h < 2; h++) {
+                key[h] = __ldg(reinterpret_cast<const uint4 *>(t.rec + t.chunk * 1024 + h * 512 + lane * 16));
+                dim[h] = __ldg(reinterpret_cast<const uint4 *>(t.rec + v_byte(t.chunk * kChunk, lane + 32 * h)));
+            }
+        }
 #pragma unroll
-                for (int j = 0; j < 4; j++) b[h][j] = turn[(4 * ((lane >> 2) + 8 * h) + j) * 4 + q];
-                turn4(b[h]);
+        for (int j = 0; j < 4; j++) {
+            const int p = 4 * j + (lane >> 3);
+            scale[0][j] = scale[1][j] = 0.0f;
+            if (p >= t.from && p < t.to) {
+                const int row = kv_row(s, t, p), place = s.place[row];
+                const uint8_t *rec = s.rec[row];
+                if (rec) {
+                    rec += (size_t)head * kKvBlockBytes;
+                    scale[0][j] = __ldg(reinterpret_cast<const float *>(rec + kKScaleOffset) + k_scale_index(place));
+                    scale[1][j] = __ldg(reinterpret_cast<const float *>(rec + kVScaleOffset) + v_scale_index(place));
+                } else if (s.bad[row]) {  // NaN; a padding row gives zeros
+                    scale[0][j] = scale[1][j] = __int_as_float(0x7fc00000);
+                }
+            }
+        }
+#pragma unroll
+        for (int which = 0; which < 2; which++) {
+            __syncwarp();
+            if (t.run && which == 0) {
+                const int r = lane >> 2, c = lane & 3;
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    uint32_t *dst = turn + r * kRow + h * 8 + c;
+                    dst[0] = key[h].x, dst[8 * kRow] = key[h].y, dst[4] = key[h].z, dst[8 * kRow + 4] = key[h].w;
+                }
+            } else if (t.run) {
+                // dims as rows of 16 bytes, turned around to positions as rows
+#pragma unroll
+                for (int h = 0; h < 2; h++) *reinterpret_cast<uint4 *>(turn + (lane + 32 * h) * 4) = dim[h];
+                __syncwarp();
+                const int q = lane & 3;
+                uint32_t b[2][4];
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+#pragma unroll
+                    for (int j = 0; j < 4; j++) b[h][j] = turn[(4 * ((lane >> 2) + 8 * h) + j) * 4 + q];
+                    turn4(b[h]);
+                }
+                __syncwarp();
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) turn[(4 * q + j) * kRow + (lane >> 2) + 8 * h] = b[h][j];
+            } else {
+                // 16 lanes a single row, two rows an access (a row's key words lie in four sectors)
+                const int c = lane & 15;
+                uint32_t w[8];
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const int p = 2 * j + (lane >> 4);
+                    const int row = p < t.to ? kv_row(s, t, p) : 0, place = s.place[row];
+                    w[j] = 0;
+                    if (p >= t.to || !s.rec[row]) continue;
+                    const uint8_t *rec = s.rec[row] + (size_t)head * kKvBlockBytes;
+                    if (which == 0) w[j] = __ldg(reinterpret_cast<const uint32_t *>(rec + k_byte(place, 4 * c)));
+                    else
+#pragma unroll
+                        for (int e = 0; e < 4; e++) w[j] |= (uint32_t)__ldg(rec + v_byte(place, 4 * c + e)) << (8 * e);
+                }
+#pragma unroll
+                for (int j = 0; j < 8; j++) turn[(2 * j + (lane >> 4)) * kRow + c] = w[j];
             }
             __syncwarp();
+            T *out = static_cast<T *>(which ? a.v_out : a.k_out);
+            const long long stride = which ? a.v_stride : a.k_stride;
 #pragma unroll
-            for (int h = 0; h < 2; h++)
-#pragma unroll
-                for (int j = 0; j < 4; j++) turn[(4 * q + j) * (kTurnRow / 4) + (lane >> 2) + 8 * h] = b[h][j];
-            __syncwarp();
-#pragma unroll
-            for (int c = 0; c < 8; c++) vw[c] = turn[r * (kTurnRow / 4) + half * 8 + c];
-        } else if (t.rec) {
-#pragma unroll
-            for (int c = 0; c < 8; c++)
-                kw[c] = __ldg(reinterpret_cast<const uint32_t *>(t.rec + k_byte(t.place, 32 * half + 4 * c)));
-#pragma unroll
-            for (int j = 0; j < 32; j++) vw[j >> 2] |= (uint32_t)__ldg(t.rec + v_byte(t.place, 32 * half + j)) << (8 * (j & 3));
+            for (int j = 0; j < 4; j++) {
+                const int p = 4 * j + (lane >> 3);
+                if (p < t.from || p >= t.to) continue;
+                const uint2 w = make_uint2(turn[p * kRow + (lane & 7) * 2], turn[p * kRow + (lane & 7) * 2 + 1]);
+                Eight<T> x;
+                scale8(w, scale[which][j], x);
+                x.store(out + (size_t)(first + kv_row(s, t, p)) * stride + head * kHeadDim + (lane & 7) * 8);
+            }
         }
-        if (!t.mine) continue;
-        float x[32];
-#pragma unroll
-        for (int j = 0; j < 32; j++) x[j] = __fmul_rn((float)(int8_t)(uint8_t)(kw[j >> 2] >> (8 * (j & 3))), ks);
-        store32(k, x);
-#pragma unroll
-        for (int j = 0; j < 32; j++) x[j] = __fmul_rn((float)(int8_t)(uint8_t)(vw[j >> 2] >> (8 * (j & 3))), vs);
-        store32(v, x);
+        __syncwarp();
     }
 }
 

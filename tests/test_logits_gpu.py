@@ -63,7 +63,8 @@ def _want(c, mask_index=None):
 
 
 @pytest.mark.parametrize("rows,vocab,tokens,bias", [(1, 1, 3, 1), (3, 31, 50, 4), (2, 4096, 300, 9), (4, 4097, 900, 40),
-                                                    (5, 8192, 2000, 100), (2, 51865, 500, 30), (7, 333, 0, 0)])
+                                                    (5, 8192, 2000, 100), (2, 51865, 500, 30), (7, 333, 0, 0),
+                                                    (21, 51865, 400, 60), (40, 30001, 6000, 900)])
 def test_logits_match_the_definition(ops, cuda, rows, vocab, tokens, bias):
     c = _case(rows + vocab, rows, vocab, tokens, bias)
     assert np.array_equal(_run(ops, cuda, c).cpu().numpy(), _want(c))
@@ -114,6 +115,36 @@ def test_each_part_alone_and_none(ops, cuda):
     assert torch.equal(got, want)
 
 
+def test_large_calls_in_place_and_unaligned(ops, cuda):
+    """The two-kernel form: in place, rows that lie differently to 16 bytes in and out, and a captured call."""
+    c = _case(12, 12, 90001, 300, 40)
+    want = _want(c)
+    wide = torch.full((12, 90007), 2.5, device=cuda)
+    wide[:, 2:90003] = torch.from_numpy(c["x"]).to(cuda)
+    out = torch.full((12, 90010), 1.5, device=cuda)
+    _run(ops, cuda, c, logits=wide[:, 2:90003], out=out[:, 1:90002])
+    assert np.array_equal(out[:, 1:90002].cpu().numpy(), want)
+    assert torch.all(out[:, :1] == 1.5) and torch.all(out[:, 90002:] == 1.5)
+    x = torch.from_numpy(c["x"]).to(cuda)
+    _run(ops, cuda, c, logits=x, out=x)
+    assert np.array_equal(x.cpu().numpy(), want)
+    x.copy_(torch.from_numpy(c["x"]))
+    mask = torch.from_numpy(c["mask"].view(np.int32)).to(cuda)
+    tok = dict(tokens=_i32([t for r in c["tokens"] for t in r], cuda), token_offsets=_i32(_offsets(c["tokens"]), cuda),
+               repetition=_f32(c["repetition"], cuda), mask=mask)
+    want = ops.logits_process(x, **tok)
+    y = torch.empty_like(x)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        ops.logits_process(x, out=y, **tok)
+    for _ in range(2):
+        y.fill_(0.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, want)
+
+
 def test_in_place_strided_and_unaligned_rows(ops, cuda):
     """In place, with row strides no vector load divides, and from an odd start."""
     c = _case(8, 3, 1001, 200, 10)
@@ -130,7 +161,19 @@ def test_in_place_strided_and_unaligned_rows(ops, cuda):
     assert torch.all(wide[:, :13] == 2.5) and torch.all(wide[:, 1014:] == 2.5)
 
 
-def test_bad_mask_rows(ops, cuda):
+@pytest.mark.parametrize("rows,vocab", [(3, 300), (150, 8190)])
+def test_bad_mask_rows(ops, cuda, rows, vocab):
+    """A mask row past the last gives a NaN row with status 2, in the small form and the large one."""
+    if rows > 3:
+        x = torch.randn((rows, vocab), device=cuda)
+        status = torch.zeros(1, dtype=torch.int32, device=cuda)
+        mask = torch.full((2, 256), -1, dtype=torch.int32, device=cuda)
+        got = ops.logits_process(x, tokens=_i32([1, 2], cuda), token_offsets=_i32([0] * 8 + [2] * (rows - 7), cuda),
+                                 presence=torch.ones(rows, device=cuda), mask=mask, mask_index=_i32([0] * 7 + [2] + [1] * (rows - 8), cuda),
+                                 status=status)
+        assert status.item() == 2 and torch.isnan(got[7]).all()
+        assert torch.equal(got[:7], x[:7]) and torch.equal(got[8:], x[8:])
+        return
     c = _case(9, 3, 300, 20, 2)
     status = torch.zeros(1, dtype=torch.int32, device=cuda)
     got = _run(ops, cuda, c, mask_index=[2, 3, -4], status=status)
