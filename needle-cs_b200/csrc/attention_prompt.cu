@@ -69,7 +69,8 @@ struct Step {
     static constexpr int kThreads = 32 * (kMmaWarp + 4);
     // Registers a thread: what the launch gives each (128 or 96), shared out anew: the softmax warps hold a row's scores.
     static constexpr int kLaunchRegs = kTiles == 2 ? 128 : 96;
-    static constexpr int kSoftmaxRegs = kTiles == 2 ? 184 : 120, kConvertRegs = kTiles == 2 ? 96 : 72, kMmaRegs = 48;
+    static constexpr int kSoftmaxRegs = kTiles == 2 ? 184 : 128, kConvertRegs = kTiles == 2 ? 96 : 64;
+    static constexpr int kMmaRegs = kTiles == 2 ? 48 : 32;
     static_assert(kTiles * kSoftmaxRegs + kConvertRegs + kMmaRegs == (kTiles + 2) * kLaunchRegs, "the launch's registers");
 };
 
@@ -96,8 +97,10 @@ struct PromptSmem {
     uint64_t raw_full[St::kRaw], kv_full[St::kStages], kv_empty[St::kStages];
     int missing[St::kRaw];  // bit g: the step's page g is not in the pool
     uint64_t s_full[St::kTiles], s_free[St::kTiles], p_full[St::kTiles], pv_done[St::kTiles];
+    uint64_t q_full;
     uint32_t tmem;
-    int seq, tile;  // this CTA's work: sequence (-1: none) and the kRows-row tile of it
+    // this CTA's work: a sequence (rows 0: none) and the kRows-row tile of it
+    int first_row, rows, slot, pos, tile;
     volatile int abort;
 };
 
@@ -149,13 +152,20 @@ __global__ void __launch_bounds__(Step<T>::kThreads, 1) attention_prompt_kernel(
 
     // This CTA's tile: sequences hold ceil(rows * group / kCtaRows) tiles each.
     if (warp == 0) {
-        int seq = -1, tile = 0, before = 0;
-        for (int base = 0; base < a.sequences && seq < 0; base += 32) {
+        bool found = false;
+        if (lane == 0) s.first_row = s.rows = s.slot = s.pos = s.tile = 0, s.abort = 0;
+        __syncwarp();  // before the lane that finds the work
+        int before = 0;
+        for (int base = 0; base < a.sequences && !found; base += 32) {
             const int i = base + lane;
-            int tiles = 0;
+            int first = 0, n = 0, slot = 0, pos = 0, tiles = 0;
             if (i < a.sequences) {
                 const int b = a.seq_rows[i], e = a.seq_rows[i + 1];
-                if (b >= 0 && e >= b && e <= a.rows) tiles = (int)(((long long)(e - b) * group + kCtaRows - 1) / kCtaRows);
+                slot = a.seq_slot[i], pos = a.seq_pos[i];
+                if (b >= 0 && e >= b && e <= a.rows) {
+                    first = b, n = e - b;
+                    tiles = (int)(((long long)n * group + kCtaRows - 1) / kCtaRows);
+                }
             }
             int sum = tiles;
 #pragma unroll
@@ -163,17 +173,14 @@ __global__ void __launch_bounds__(Step<T>::kThreads, 1) attention_prompt_kernel(
                 const int up = __shfl_up_sync(0xffffffffu, sum, o);
                 if (lane >= o) sum += up;
             }
-            const bool mine = work >= before + sum - tiles && work < before + sum;
-            const unsigned who = __ballot_sync(0xffffffffu, mine);
-            if (who) {
-                const int l = __ffs(who) - 1;
-                seq = base + l;
-                // the last tile, which sees the most pages, first
-                tile = __shfl_sync(0xffffffffu, tiles - 1 - (work - (before + sum - tiles)), l);
+            const int at = work - (before + sum - tiles);
+            const bool mine = at >= 0 && at < tiles;
+            if (mine) {  // the last tile, which sees the most pages, first
+                s.first_row = first, s.rows = n, s.slot = slot, s.pos = pos, s.tile = tiles - 1 - at;
             }
+            found = __any_sync(0xffffffffu, mine);
             before += __shfl_sync(0xffffffffu, sum, 31);
         }
-        if (lane == 0) s.seq = seq, s.tile = tile, s.abort = 0;
         if (blockIdx.x == 0)
             for (int i = lane; i < a.sequences; i += 32) {
                 const int b = a.seq_rows[i], e = a.seq_rows[i + 1];
@@ -181,6 +188,7 @@ __global__ void __launch_bounds__(Step<T>::kThreads, 1) attention_prompt_kernel(
             }
     } else if (warp == kMmaWarp) {
         if (lane == 0) {
+            mbar_init(&s.q_full, 4 * kTiles);
             for (int i = 0; i < St::kRaw; i++) mbar_init(&s.raw_full[i], 1);
             for (int i = 0; i < kStages; i++) mbar_init(&s.kv_full[i], kConvertWarps), mbar_init(&s.kv_empty[i], kTiles);
             for (int t = 0; t < kTiles; t++)
@@ -196,21 +204,19 @@ __global__ void __launch_bounds__(Step<T>::kThreads, 1) attention_prompt_kernel(
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = s.tmem;
-    const int seq = s.seq;
-    const int first_row = seq >= 0 ? a.seq_rows[seq] : 0;
-    const int n = seq >= 0 ? a.seq_rows[seq + 1] - first_row : 0;
-    const int slot = seq >= 0 ? a.seq_slot[seq] : 0, start = seq >= 0 ? a.seq_pos[seq] : 0;
+    const int n = s.rows, first_row = s.first_row, slot = s.slot, start = s.pos;
     const bool ok_seq = slot >= 0 && slot < a.c.slots && start >= 0 &&
                         (long long)start + n <= (long long)a.c.max_pages * kPagePositions;
-    const long long packed = (long long)n * group, m0 = (long long)s.tile * kCtaRows;
+    // (rows x heads is below 2^31)
+    const unsigned packed = (unsigned)n * group, m0 = (unsigned)s.tile * kCtaRows;
     // the pages its rows see, from page0 on in steps; steps [lo, hi] of each tile (hi < lo: no rows)
     int lo[kTiles], hi[kTiles], page0 = 0, steps = 0;
 #pragma unroll
     for (int t = 0; t < kTiles; t++) {
-        const long long b = m0 + t * kTileRows, e = min(packed, b + kTileRows);
+        const unsigned b = m0 + t * kTileRows, e = min(packed, b + kTileRows);
         lo[t] = 0, hi[t] = -1;
-        if (seq >= 0 && ok_seq && b < e) {
-            const int from = start + (int)(b / group), to = start + (int)((e - 1) / group);
+        if (n > 0 && ok_seq && b < e) {
+            const int from = start + (int)(b / (unsigned)group), to = start + (int)((e - 1) / (unsigned)group);
             const int first = a.window ? max(0, from - a.window + 1) / kPagePositions : 0;
             if (t == 0) page0 = first;
             lo[t] = (first - page0) / kPages;
@@ -220,16 +226,17 @@ __global__ void __launch_bounds__(Step<T>::kThreads, 1) attention_prompt_kernel(
     }
     // a warp's tile, and the steps it takes
     const auto pick = [&](const int(&x)[kTiles], int t) { return t == 0 ? x[0] : t == 1 ? x[1] : x[kTiles - 1]; };
-    const int last_pos = start + (int)((min(packed, m0 + kCtaRows) - 1) / group);  // the CTA's last query
+    const int last_pos = start + (int)((max(1u, min(packed, m0 + kCtaRows)) - 1) / (unsigned)group);  // the CTA's last query
 
     if (warp < St::kConvertWarp) {
         // ------------------------------------------------------- softmax --
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(St::kSoftmaxRegs));
         const int t = warp >> 2, row = threadIdx.x & (kTileRows - 1);
         const int lo_t = pick(lo, t), hi_t = pick(hi, t);
-        const long long m = m0 + t * kTileRows + row;
-        const bool valid = seq >= 0 && m < packed;
-        const int query = valid ? (int)(m / group) : 0, head = kv_head * group + (valid ? (int)(m % group) : 0);
+        const unsigned m = m0 + t * kTileRows + row;
+        const bool valid = m < packed;  // (no work: packed is 0)
+        const int query = valid ? (int)(m / (unsigned)group) : 0;
+        const int head = kv_head * group + (valid ? (int)(m - (unsigned)query * group) : 0);
         const size_t at = (size_t)(first_row + query);
         const int pos = start + query;
         float scale_q = 1.0f;
@@ -263,7 +270,8 @@ __global__ void __launch_bounds__(Step<T>::kThreads, 1) attention_prompt_kernel(
             }
         }
         fence_proxy_async_smem();
-        __syncthreads();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s.q_full);
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t ts = tmem + lanes + St::kS + t * kCols, to = tmem + lanes + St::kO + t * kHeadDim;
         const uint32_t tp = tmem + lanes + St::kP + t * St::kPCols;
@@ -401,7 +409,6 @@ __global__ void __launch_bounds__(Step<T>::kThreads, 1) attention_prompt_kernel(
         const int c = warp - St::kConvertWarp;
         int exponent = kMinExponent;
         const float fold = a.scale * kLog2E;
-        __syncthreads();
         for (int i = 0; i < steps; i++) {
             const int st = i % kStages, rs = i % St::kRaw;
             if (!warp_wait(&s.raw_full[rs], (i / St::kRaw) & 1, &s.abort) ||
@@ -517,7 +524,6 @@ __global__ void __launch_bounds__(Step<T>::kThreads, 1) attention_prompt_kernel(
     } else {
         // ------------------------------------------------------ MMA issuer --
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(St::kMmaRegs));
-        __syncthreads();
         bool ok = true;
         if (warp == St::kCopyWarp) {
             // the records of each step into their ring, once the converters have read the step kRaw before
@@ -578,6 +584,7 @@ __global__ void __launch_bounds__(Step<T>::kThreads, 1) attention_prompt_kernel(
                 mma_commit_elect(&s.s_full[t]);
                 if (lane == 0) mbar_arrive(&s.s_full[t]);
             };
+            if (steps > 0) ok = warp_wait(&s.q_full, 0, &s.abort);
             scores(0);
             for (int i = 0; i < steps && ok; i++) {
                 scores(i + 1);
