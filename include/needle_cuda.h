@@ -247,9 +247,11 @@ NDL_API int ndl_kv_gather(const int32_t *row_slot, const int32_t *row_pos, int r
  * head h reads kv head h / (heads / kv_heads).  With window w > 0 a query at
  * position p attends to (p - w, p], else to [0, p]:
  *   out = sum_j softmax_j(scale * q . k_j) v_j
- * Scores, softmax and sums are in fp32; 16-bit types round the
- * probabilities to fp16 before the second product, fp32 splits queries and
- * probabilities into two fp16 parts.  Rows of no sequence are left as they
+ * Scores, softmax and sums are in fp32.  The products' operands are fp16,
+ * scaled by powers of two: for bf16 keys, values (code * scale) and
+ * probabilities round to one each; for fp16 the keys have two parts and the
+ * value scales go to the probabilities; for fp32 queries and probabilities
+ * have two parts too.  out may be q.  Rows of no sequence are left as they
  * are; a sequence whose offsets descend or leave [0, rows] is skipped with
  * status 2, and so may be those behind it. */
 NDL_API int ndl_attention_prompt(const void *q, long long q_stride, int type, const int32_t *seq_rows,
@@ -261,7 +263,9 @@ NDL_API int ndl_attention_prompt(const void *q, long long q_stride, int type, co
 /* Attention of single tokens: row r attends to positions [0, row_len[r]) of
  * slot row_slot[r] (the last `window` of them with window > 0), its cache
  * split over several thread blocks and the parts joined.  A row of length 0
- * gives zeros.  Arithmetic as ndl_attention_prompt.  workspace: device
+ * gives zeros.  Arithmetic as ndl_attention_prompt, but for the operands:
+ * codes are exact in them, the key scales multiply scores, the value scales
+ * probabilities, for every type.  out may be q.  workspace: device
  * memory of ndl_attention_split_workspace bytes, 16-byte aligned; calls that
  * overlap on the GPU need one each.  Its contents need no set-up and mean
  * nothing between calls. */
@@ -286,7 +290,8 @@ NDL_API int ndl_attention_split(const void *q, long long q_stride, int type, con
  * entries bias_ids / bias_values [bias_offsets[r] .. bias_offsets[r+1]); ids
  * outside the vocabulary are ignored.  Its mask is masks' row mask_index[r]
  * (negative: none), without mask_index row r; a row past mask_rows is NaN
- * with status 2.  Every list and penalty is nullable. */
+ * with status 2.  Every list and penalty is nullable.  At most 65535 rows and
+ * 2^30 ids. */
 NDL_API int ndl_logits_process(const float *x, long long ldx, float *y, long long ldy, int rows, int vocab,
                                const int32_t *tokens, int n_tokens, const int32_t *token_offsets,
                                const int32_t *prompt_lens, const float *repetition, const float *frequency,

@@ -395,6 +395,77 @@ def test_attention_wrapper_refusals(ops, cuda):
         ops.attention_split(torch.zeros((1, 5, 64), device=cuda), one, one, 2, *pages)
 
 
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_outputs_in_the_queries_place(ops, cuda, kind):
+    """out may be q: rows inside a warp, over a CTA's warps and over CTAs, and a prompt of several tiles."""
+    cache = Cache(61, [9000, 700, 65, 3], 2)
+    lengths = cache.lengths
+    q, _ = _queries(cache, kind, 4, 8, cuda)
+    args = (_i32(range(4), cuda), _i32(lengths, cuda), 2, *cache.device(cuda))
+    want = ops.attention_split(q, *args)
+    assert ops.attention_split(q, *args, out=q) is q
+    assert torch.equal(q, want)
+    q, _ = _queries(cache, kind, 1000, 8, cuda)
+    args = (_i32([0, 700, 990, 1000], cuda), _i32([1, 0, 2], cuda), _i32([0, 8000, 55], cuda), 2, *cache.device(cuda))
+    want = ops.attention_prompt(q, *args)
+    assert ops.attention_prompt(q, *args, out=q) is q
+    assert torch.equal(q, want)
+
+
+def test_windows_of_any_size(ops, cuda):
+    """A window longer than the sequence is none, up to the largest int."""
+    cache = Cache(62, [1500, 3], 2)
+    q, _ = _queries(cache, "bf16", 600, 4, cuda)
+    args = (_i32([0, 597, 600], cuda), _i32([0, 1], cuda), _i32([903, 0], cuda), 2, *cache.device(cuda))
+    single = (_i32([0, 1], cuda), _i32([1500, 3], cuda), 2, *cache.device(cuda))
+    want, want_split = ops.attention_prompt(q, *args), ops.attention_split(q[:2], *single)
+    for window in (1500, 1 << 20, 2 ** 31 - 1):
+        assert torch.equal(ops.attention_prompt(q, *args, window=window), want)
+        assert torch.equal(ops.attention_split(q[:2], *single, window=window), want_split)
+
+
+def test_two_calls_at_once(ops, cuda):
+    """The same rows on two streams, each with its own workspace and pages of one pool."""
+    cache = Cache(63, [4000, 300, 3000, 64], 2)
+    table, pool, page_bytes, layer = cache.device(cuda)
+    q, _ = _queries(cache, "f16", 4, 8, cuda)
+    slots, lengths = _i32(range(4), cuda), _i32(cache.lengths, cuda)
+    want = ops.attention_split(q, slots, lengths, 2, table, pool, page_bytes, layer)
+    prompt = (_i32([0, 4], cuda), _i32([2], cuda), _i32([2996], cuda), 2, table, pool, page_bytes, layer)
+    want_prompt = ops.attention_prompt(q, *prompt)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(10):
+        for stream in streams:
+            with torch.cuda.stream(stream):
+                got.append((ops.attention_split(q, slots, lengths, 2, table, pool, page_bytes, layer),
+                            ops.attention_prompt(q, *prompt)))
+    torch.cuda.synchronize()
+    for split, prompted in got:
+        assert torch.equal(split, want) and torch.equal(prompted, want_prompt)
+
+
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="one GPU")
+def test_a_device_that_is_not_current(ops, cuda):
+    """The tensors' device decides, whichever is current; its kernels' attributes are set there too."""
+    cache = Cache(64, [700, 90], 2)
+    other = torch.device("cuda", 1)
+    results = []
+    for device in (cuda, other):
+        q = torch.from_numpy(np.random.default_rng(5).normal(size=(2, 8, 64))).float().to(device)
+        pages = cache.device(device)
+        slots = torch.tensor([0, 1], dtype=torch.int32, device=device)
+        lengths = torch.tensor([700, 90], dtype=torch.int32, device=device)
+        results.append([ops.attention_split(q, slots, lengths, 2, *pages),
+                        ops.attention_prompt(q, torch.tensor([0, 1, 2], dtype=torch.int32, device=device), slots,
+                                             lengths - 1, 2, *pages), *ops.kv_gather(slots, lengths - 1, 2, *pages),
+                        ops.logits_process(q.flatten(1))])
+    for a, b in zip(*results):
+        assert b.device == other and torch.equal(a.cpu(), b.cpu())
+
+
+
 # ----------------------------------------------------------------- together --
 
 def test_a_request_from_prompt_to_token(ops, cuda):

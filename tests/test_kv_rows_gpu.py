@@ -156,3 +156,65 @@ def test_wrapper_refusals(ops, cuda):
         ops.kv_append(k, k, _i32([0, 0], cuda), one, table, pool, page_bytes, layer)
     with pytest.raises(TypeError):
         ops.kv_append(k, k, one.long(), one, table, pool, page_bytes, layer)
+
+
+def test_many_rows_of_runs_singles_and_padding(ops, cuda):
+    """Enough rows for the larger blocks: chunks at any start, single tokens and padding, shuffled, so runs cross
+    blocks and chunks of pages; nothing else in the pool changes, and the rows come back."""
+    cache = Cache(21, [130] * 60, 3)
+    rng = np.random.default_rng(22)
+    pieces = []
+    for s in rng.permutation(60):  # each slot in pieces of 1 to 45 positions, some positions left out
+        at = int(rng.integers(0, 9))
+        while at < 130:
+            n = int(rng.integers(1, 46)) if rng.random() < 0.7 else 1
+            pieces.append([(s, p) for p in range(at, min(130, at + n))])
+            at += n + int(rng.integers(0, 3))
+    places = []
+    for i in rng.permutation(len(pieces)):
+        places += pieces[i]
+        places += [(int(rng.integers(-1, 60)), -1)] * int(rng.integers(0, 3) // 2)
+    rows = len(places)
+    assert (rows + 31) // 32 * 3 >= 296
+    k, v, x = _rows(cache, "bf16", rows, rng, cuda)
+    table, pool, page_bytes, layer = cache.device(cuda)
+    status = torch.zeros(1, dtype=torch.int32, device=cuda)
+    slot, pos = (_i32(a, cuda) for a in zip(*places))
+    ops.kv_append(k, v, slot, pos, table, pool, page_bytes, layer, status=status)
+    real = [r for r, (_, p) in enumerate(places) if p >= 0]
+    want = _expected(cache, [places[r] for r in real], x[0][real], x[1][real])
+    assert np.array_equal(pool.cpu().numpy(), want.reshape(-1))
+    for kind in TYPES:
+        got = ops.kv_gather(slot, pos, 3, table, pool, page_bytes, layer, dtype=TYPES[kind], status=status)
+        for g, r in zip(got, x):
+            codes, scales = quantized(r)
+            back = torch.from_numpy(codes.astype(np.float32) * scales[..., None]).to(TYPES[kind])
+            back[[p < 0 for _, p in places]] = 0
+            assert torch.equal(g.cpu(), back)
+    assert status.item() == 0
+
+
+def test_append_and_gather_on_a_stream_and_in_a_graph(ops, cuda):
+    """Captured on a side stream and replayed with other rows and places."""
+    cache = Cache(23, [100, 90], 2)
+    rng = np.random.default_rng(24)
+    table, pool, page_bytes, layer = cache.device(cuda)
+    k, v = torch.zeros((40, 2, 64), device=cuda), torch.zeros((40, 2, 64), device=cuda)
+    slot, pos = _i32([0] * 40, cuda), _i32([-1] * 40, cuda)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        ops.kv_append(k, v, slot, pos, table, pool, page_bytes, layer)
+        back = ops.kv_gather(slot, pos, 2, table, pool, page_bytes, layer)
+    for _ in range(3):
+        places = _places(cache, rng, 25) + [(0, -1)] * 15
+        x = rng.normal(size=(2, 40, 2, 64)).astype(np.float32)
+        for t, value in ((k, x[0]), (v, x[1]), (slot, [s for s, _ in places]), (pos, [p for _, p in places])):
+            t.copy_(torch.as_tensor(np.asarray(value)))
+        graph.replay()
+        for got, value in zip(back, x):
+            codes, scales = quantized(value)
+            want = codes.astype(np.float32) * scales[..., None]
+            want[25:] = 0
+            assert np.array_equal(got.cpu().numpy(), want)

@@ -226,3 +226,62 @@ def test_before_the_engines_sampler(ops, pkg, cuda):
         want = np.stack([processed(rows[0], bias=[(int(ids[0]), -1e4)]), processed(rows[1], bias=[(17, 1e4)])])
         assert np.array_equal(got.cpu().numpy(), want)
         assert got.argmax(1).tolist()[1] == 17 and got.argmax(1).tolist()[0] != ids[0]
+
+
+def test_many_ids_in_place_unaligned_and_in_a_graph(ops, cuda):
+    """Calls of millions of ids: in place, rows that lie differently to 16 bytes in and out, one row with lists too
+    long for shared memory, one whose mask does not exist, and a captured call."""
+    rows, vocab = 40, 90001
+    c = _case(16, rows, vocab, 300, 40)
+    c["tokens"][3] = [(i * i) % (vocab + 7) for i in range(9000)]
+    c["prompt"][3] = 4000
+    c["bias"][3] = [((31 * i) % vocab, float(np.float32(0.01 * i))) for i in range(500)]
+    want = _want(c)
+    x = torch.from_numpy(c["x"]).to(cuda)
+    wide = torch.full((rows, vocab + 6), 2.5, device=cuda)
+    wide[:, 2:vocab + 2] = x
+    out = torch.full((rows, vocab + 9), 1.5, device=cuda)
+    _run(ops, cuda, c, logits=wide[:, 2:vocab + 2], out=out[:, 1:vocab + 1])
+    assert np.array_equal(out[:, 1:vocab + 1].cpu().numpy(), want)
+    assert torch.all(out[:, :1] == 1.5) and torch.all(out[:, vocab + 1:] == 1.5)
+    y = x.clone()
+    _run(ops, cuda, c, logits=y, out=y)
+    assert np.array_equal(y.cpu().numpy(), want)
+    status = torch.zeros(1, dtype=torch.int32, device=cuda)
+    index = list(range(rows))
+    index[7] = rows
+    got = _run(ops, cuda, c, mask_index=index, status=status)
+    assert status.item() == 2 and torch.isnan(got[7]).all()
+    keep = [r for r in range(rows) if r != 7]
+    assert np.array_equal(got[keep].cpu().numpy(), want[keep])
+    mask = torch.from_numpy(c["mask"].view(np.int32)).to(cuda)
+    tok = dict(tokens=_i32([t for r in c["tokens"] for t in r], cuda), token_offsets=_i32(_offsets(c["tokens"]), cuda),
+               repetition=_f32(c["repetition"], cuda), mask=mask)
+    eager = ops.logits_process(x, **tok)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        ops.logits_process(x, out=y, **tok)
+    for _ in range(2):
+        y.fill_(0.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, eager)
+
+
+def test_large_calls_whose_lists_are_empty(ops, cuda):
+    """What follows on the stream reads the whole result, although no row's list has work."""
+    rows, vocab = 128, 1 << 15
+    x = torch.randn((rows, vocab), device=cuda)
+    zero = torch.zeros(rows + 1, dtype=torch.int32, device=cuda)
+    some = _i32([1, 2, 3], cuda)
+    mask = torch.full((rows, vocab // 32), 0x0F0F0F0F, dtype=torch.int32, device=cuda)
+    allowed = (torch.arange(vocab, device=cuda) & 4) == 0
+    want = torch.where(allowed, x, torch.full_like(x, -torch.inf))
+    out = torch.zeros_like(x)
+    torch.cuda.synchronize()
+    for _ in range(20):
+        out.zero_()
+        ops.logits_process(x, out=out, tokens=some, token_offsets=zero, repetition=torch.ones(rows, device=cuda), mask=mask)
+        copy = out.clone()
+        assert torch.equal(copy, want)
