@@ -1,11 +1,11 @@
 // Whole-prompt attention over the paged int8 cache, on the fifth-generation
 // tensor cores.
 //
-// A CTA takes 256 packed rows (two tiles of 128) of one sequence and kv head;
-// packed row m is query m / group of the sequence and query head m % group of
-// the kv head's group, so a page of keys and values serves every query head
-// that shares it.  It walks the pages its rows see, 128 positions a step
-// (fp32: 64), with the softmax's running maximum and sum:
+// A CTA takes up to 384 packed rows (three tiles of 128; fp32: two) of one
+// sequence and kv head; packed row m is query m / group of the sequence and
+// query head m % group of the kv head's group, so a page of keys and values
+// serves every query head that shares it.  It walks the pages its rows see, one
+// (64 positions) a step, with the softmax's running maximum and sum:
 //   S = Q K^T       tcgen05.mma, fp16 operands, fp32 accumulator in TMEM
 //   e = 2^(f S - m),  l += e,  P = e,  O += P V
 // Every operand is brought into fp16's range by a power of two: a query row's
@@ -19,15 +19,25 @@
 //   fp16  keys in two parts (22 bits), values as bare codes (exact) with their
 //         scales on P, which rounds as the result does;
 //   fp32  as fp16, and queries and P in two parts: 2^-21 throughout.
-// The scales go into the operands because a scale a column costs the softmax
+// The key scales go into the operand because a scale a column costs the softmax
 // threads (thread = row) a shared-memory wavefront a column and warp: with both
-// scales there the pipe was as busy as the exponentials (967 us for 8192 rows
-// of 32 heads over 8).
+// scales there that pipe was as busy as the exponentials (8192 rows of 32 heads
+// over 8: 967 us then, 730 with the scales in the operands).
 //
 // Warps: 4 softmax warps a tile (maximum and sum need no exchange), 4 that
-// convert pages (int8 records -> fp16 tiles in shared memory, 128-byte
-// swizzled rows), 1 that copies the records, 1 a tile that issues its MMAs.  P goes back to TMEM, from where the
-// second product takes it as its A operand.
+// convert pages (int8 records -> fp16 tiles in shared memory, 128-byte swizzled
+// rows), 1 that copies the records, 1 a tile that issues its MMAs.  P goes back
+// to TMEM, from where the second product takes it as its A operand.
+//
+// Bound by the softmax warps: a column costs a row an exponential (16 a clock
+// and SM) and some six instructions more.  8192 rows of 32 heads over 8, bf16,
+// causal: 461 us (0.60 PFLOP/s), where the two products alone would take 163 at
+// the library's rate; of 478 it took 434 without the exponentials and 473 without
+// the conversions.  The three tiles hide one another's waits: two took 524, two
+// with steps of 128 columns 545, one tile and two CTAs an SM 664.  Short prompts
+// are bound by what a CTA does around its steps (a step of three tiles takes 1.4
+// us, of fp32's two 1.6, all else 9 to 11) and by the CTAs that come last: 32
+// prompts of up to 384 rows, 8 heads, fp32: 40 us; one of 37 rows: 8 us.
 //
 // A value scale that is no number would reach rows that do not see its
 // position through the product (0 * NaN): it is replaced by 0 and its key
@@ -54,9 +64,10 @@ struct Step {
     static constexpr bool kSplit = sizeof(T) == 4;                       // queries and P in two parts
     static constexpr bool kFoldValues = __is_same(T, __nv_bfloat16);     // value scales on the values, else on P
     static constexpr int kQParts = kSplit ? 2 : 1, kKParts = kFoldValues ? 1 : 2;
-    // Tiles of 128 rows: three, whose softmax warps pass their waits under one another's exponentials; the second
-    // parts of fp32 leave TMEM room for two.
+    // Tiles of 128 rows: three (above); the softmax of fp32, with a second part of each probability, needs the
+    // registers of two.
     static constexpr int kTiles = kSplit ? 2 : 3, kRows = kTiles * kTileRows;
+    // Pages a step: one; with two the scores' registers spill or leave room for two tiles alone (above).
     static constexpr int kPages = 1, kCols = kPages * kPagePositions;
     static constexpr int kStages = 4;  // converted steps in flight
     static constexpr int kRaw = 3;     // steps of records as they lie in the pages
@@ -67,6 +78,9 @@ struct Step {
     // Warps: softmax, converters, then a group of one MMA warp a tile and one that copies.
     static constexpr int kConvertWarp = 4 * kTiles, kMmaWarp = kConvertWarp + kConvertWarps, kCopyWarp = kMmaWarp + 3;
     static constexpr int kThreads = 32 * (kMmaWarp + 4);
+    // 16-byte chunks of a query row, and the row (of a warp's 32) whose chunk lane % kRowChunks access i takes.
+    static constexpr int kRowChunks = kHeadDim * (int)sizeof(T) / 16;
+    __device__ static constexpr int chunk_row(int i, int lane) { return i * (32 / kRowChunks) + lane / kRowChunks; }
     // Registers a thread: what the launch gives each (128 or 96), shared out anew: the softmax warps hold a row's scores.
     static constexpr int kLaunchRegs = kTiles == 2 ? 128 : 96;
     static constexpr int kSoftmaxRegs = kTiles == 2 ? 184 : 128, kConvertRegs = kTiles == 2 ? 96 : 64;
@@ -97,12 +111,24 @@ struct PromptSmem {
     uint64_t raw_full[St::kRaw], kv_full[St::kStages], kv_empty[St::kStages];
     int missing[St::kRaw];  // bit g: the step's page g is not in the pool
     uint64_t s_full[St::kTiles], s_free[St::kTiles], p_full[St::kTiles], pv_done[St::kTiles];
-    uint64_t q_full;
+    uint64_t q_full, drained[St::kTiles];
     uint32_t tmem;
     // this CTA's work: a sequence (rows 0: none) and the kRows-row tile of it
     int first_row, rows, slot, pos, tile;
     volatile int abort;
 };
+
+// Where 16-byte chunk j of a tile's row lies before it is normalised and after it is attended: in the swizzled rows of
+// the query tiles (fp32: the second eight chunks in the second part's).
+template <class T>
+__device__ __forceinline__ uint8_t *row_chunk(PromptSmem<T> &s, int tile, int row, int j) {
+    return &s.q[tile][j >> 3][row * 128 + (((j & 7) ^ (row & 7)) << 4)];
+}
+// 16 bytes to shared memory, zeros unless they are `there` (the address is valid all the same).
+__device__ __forceinline__ void async_chunk(void *dst, const void *src, bool there) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(there ? 16 : 0)
+                 : "memory");
+}
 
 // kind::f16, fp32 accumulator, A and B fp16, both K-major.
 constexpr uint32_t idesc_f16(int m, int n) {
@@ -189,6 +215,7 @@ __global__ void __launch_bounds__(Step<T>::kThreads, 1) attention_prompt_kernel(
     } else if (warp == kMmaWarp) {
         if (lane == 0) {
             mbar_init(&s.q_full, 4 * kTiles);
+            for (int t = 0; t < kTiles; t++) mbar_init(&s.drained[t], 1);
             for (int i = 0; i < St::kRaw; i++) mbar_init(&s.raw_full[i], 1);
             for (int i = 0; i < kStages; i++) mbar_init(&s.kv_full[i], kConvertWarps), mbar_init(&s.kv_empty[i], kTiles);
             for (int t = 0; t < kTiles; t++)
@@ -241,16 +268,28 @@ __global__ void __launch_bounds__(Step<T>::kThreads, 1) attention_prompt_kernel(
         const int pos = start + query;
         float scale_q = 1.0f;
         if (hi_t >= lo_t) {
-            // the query row: normalised to fp16 (in two parts), dims in the
-            // order the key tiles have them, into the swizzled A tile
-            const T *src = static_cast<const T *>(a.q) + at * a.q_stride + (size_t)head * kHeadDim;
+            // the query row: normalised to fp16 (in two parts), dims in the order the key tiles have them, into the
+            // swizzled A tile.  A warp's rows come in whole sectors, through the tile's own place (thread = row would
+            // take a line a lane and access; there and for the results that was 4 us of a CTA's 20).
+            const uint64_t src = valid ? (uint64_t)(static_cast<const T *>(a.q) + at * a.q_stride + (size_t)head * kHeadDim) : 0;
+#pragma unroll
+            for (int i = 0; i < St::kRowChunks; i++) {
+                const uint64_t from = __shfl_sync(0xffffffffu, src, St::chunk_row(i, lane));
+                async_chunk(row_chunk(s, t, (warp & 3) * 32 + St::chunk_row(i, lane), lane % St::kRowChunks),
+                            from ? reinterpret_cast<const uint8_t *>(from) + lane % St::kRowChunks * 16 : a.q, from != 0);
+            }
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            __syncwarp();
             float x[kHeadDim], peak = 0.0f;
 #pragma unroll
-            for (int i = 0; i < kHeadDim; i += 4) {
-                float f[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                if (valid) load4(src + i, f);
+            for (int j = 0; j < St::kRowChunks; j++) {
+                constexpr int kPer = 16 / (int)sizeof(T);
+                const uint4 w = *reinterpret_cast<const uint4 *>(row_chunk(s, t, row, j));
 #pragma unroll
-                for (int j = 0; j < 4; j++) x[i + j] = f[j], peak = fmaxf(peak, fabsf(f[j]));
+                for (int e = 0; e < kPer; e++) {
+                    const float f = to_float(reinterpret_cast<const T *>(&w)[e]);
+                    x[j * kPer + e] = f, peak = fmaxf(peak, fabsf(f));
+                }
             }
             float up;
             query_norm(peak, up, scale_q);
@@ -281,7 +320,7 @@ __global__ void __launch_bounds__(Step<T>::kThreads, 1) attention_prompt_kernel(
         for (int i = lo_t; i <= hi_t; i++) {
             const int it = i - lo_t, st = i % kStages;
             // positions [from, upto] of the step are this row's
-            const int upto = pos - (page0 + i * kPages) * kPagePositions;
+            const int upto = max(pos - (page0 + i * kPages) * kPagePositions, -1);
             const int from = a.window ? upto - a.window + 1 : 0;
             const bool whole = __all_sync(0xffffffffu, upto >= kCols - 1 && from <= 0);
             ok = warp_wait(&s.s_full[t], it & 1, &s.abort);
@@ -382,17 +421,25 @@ __global__ void __launch_bounds__(Step<T>::kThreads, 1) attention_prompt_kernel(
             tmem_ld32(to + 32, r1);
             tmem_ld_wait(r0);
             tmem_ld_wait(r1);
-            if (valid) {
-                const float inverse = ok ? 1.0f / total : __int_as_float(0x7fc00000), back = pow2(exponent - 8);
-                float x[64];
+            const float inverse = ok ? 1.0f / total : __int_as_float(0x7fc00000), back = pow2(exponent - 8);
+            float x[64];
 #pragma unroll
-                for (int j = 0; j < 32; j++) {
-                    x[j] = __uint_as_float(r0[j]) * inverse * back;
-                    x[j + 32] = __uint_as_float(r1[j]) * inverse * back;
-                }
-                T *dst = static_cast<T *>(a.out) + at * a.out_stride + (size_t)head * kHeadDim;
+            for (int j = 0; j < 32; j++) {
+                x[j] = __uint_as_float(r0[j]) * inverse * back;
+                x[j + 32] = __uint_as_float(r1[j]) * inverse * back;
+            }
+            // through the queries' place, whose products have ended, to whole sectors again
 #pragma unroll
-                for (int j = 0; j < 64; j += 16 / (int)sizeof(T)) store16(dst + j, x + j);
+            for (int j = 0; j < St::kRowChunks; j++)
+                store16(reinterpret_cast<T *>(row_chunk(s, t, row, j)), x + j * (16 / (int)sizeof(T)));
+            __syncwarp();
+            const uint64_t dst = valid ? (uint64_t)(static_cast<T *>(a.out) + at * a.out_stride + (size_t)head * kHeadDim) : 0;
+#pragma unroll
+            for (int i = 0; i < St::kRowChunks; i++) {
+                const uint64_t to = __shfl_sync(0xffffffffu, dst, St::chunk_row(i, lane));
+                const uint4 w = *reinterpret_cast<const uint4 *>(
+                    row_chunk(s, t, (warp & 3) * 32 + St::chunk_row(i, lane), lane % St::kRowChunks));
+                if (to) reinterpret_cast<uint4 *>(to)[lane % St::kRowChunks] = w;
             }
         } else if (valid) {  // a bad sequence
             if (a.c.status) atomicOr(a.c.status, kStatusBadPage);
@@ -605,6 +652,10 @@ __global__ void __launch_bounds__(Step<T>::kThreads, 1) attention_prompt_kernel(
                     if (!ok) break;
                 }
                 mma_commit_elect(&s.kv_empty[st]);
+            }
+            if (!ok) {  // every product in flight ends before the CTA's TMEM is freed (bounded)
+                mma_commit_elect(&s.drained[t]);
+                mbar_wait_bounded(&s.drained[t], 0, kPromptWait);
             }
         }
         if (!ok) {
