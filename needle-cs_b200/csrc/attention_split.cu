@@ -18,6 +18,11 @@
 // l) meet in shared memory; those of items that reach over a CTA's records go
 // to the workspace, and a second kernel, launched early, joins them.  Pieces
 // are always taken in record order, so the result does not depend on timing.
+// A few items (one an SM) of a few pages take a CTA each instead: no look at the
+// other rows and no second kernel (8 kv heads, fp32, split and whole: 1 row of 4
+// pages 10.6 and 6.8 us, of 16 11.1 and 11.2, of 24 11.2 and 13.4; 18 rows of up
+// to 4 pages 11.2 and 7.2, 16 16.8 and 11.6, 24 17.0 and 14.2; bf16: of 16 pages
+// 10.6 and 10.1, 12.9 and 10.4).
 //
 // Bound by memory where the cache is long: 256 rows of up to 8192 positions, 8
 // kv heads, bf16: 194 us (5.6 TB/s, floor 167); heads as the products' columns, of
@@ -38,6 +43,7 @@ namespace {
 
 constexpr int kSplitStages = 2;
 constexpr int kSplitCtas = 148;                       // one CTA an SM
+constexpr int kWholePages = 16;                       // of a row: up to here a CTA takes an item, if they are few (above)
 constexpr int kHeadBlock = 16;                        // query heads an item holds
 constexpr uint32_t kSplitWait = 1u << 22;             // tests of about a microsecond: a few seconds
 // A piece: per head 64 outputs, m and l (padded to 16 bytes).
@@ -65,6 +71,7 @@ struct SplitArgs {
     const int32_t *row_slot, *row_len;
     int rows, heads, group, blocks, window;  // blocks: items a kv head and row
     int piece_heads;                         // heads a piece holds: min(group, 16)
+    bool whole;                              // a CTA an item
     float scale;
     PagedCache c;
     SplitItem *over;  // [kSplitCtas + 1]: the item at a CTA's first record if it began before (else row -1); behind
@@ -208,6 +215,7 @@ struct SplitSmem {
     SplitItem info[Sh::kWarps][2];                          // the pieces' items (row -1: no piece)
     uint64_t full[Sh::kWarps][kSplitStages];
     long long sums[Sh::kThreads + 1];
+    long long begin, end, records;                          // the CTA's records, and the call's
 };
 static_assert(kHeadBlock * kPieceHead * 4 <= kKvBlockBytes, "a piece fits a ring record");
 
@@ -374,74 +382,86 @@ __global__ void __launch_bounds__(SplitShape<kWide, sizeof(T) == 4>::kThreads, 1
     if (lane < 2) s.info[warp][lane].row = -1;
     fence_mbar_init();
     __syncwarp();
-    // Records before each row.  Up to 32 rows: every warp scans them by itself, lane = row.  More: a thread sums a run
-    // of rows, the CTA scans the runs.
-    const auto row_records = [&](int row) {
-        int first, last;
-        row_pages(a, row, first, last);
-        return (long long)(last - first) * virtual_heads;
-    };
-    const auto scan = [&](long long x) {  // over the warp, this lane included
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const long long up = __shfl_up_sync(0xffffffffu, x, o);
-            if (lane >= o) x += up;
-        }
-        return x;
-    };
     SplitCursor cur;
-    long long records, at = 0;  // at: records before the first one's row
-    long long upto = 0, mine = 0;
-    if (a.rows <= 32) {
-        mine = lane < a.rows ? row_records(lane) : 0, upto = scan(mine);
-        records = __shfl_sync(0xffffffffu, upto, 31);
-    } else {
-        const int run = (a.rows + kThreads - 1) / kThreads;
-        for (int i = threadIdx.x * run; i < min(a.rows, (int)(threadIdx.x + 1) * run); i++) mine += row_records(i);
-        const long long sum = scan(mine);
-        if (lane == 31) s.sums[warp + 1] = sum;
-        __syncthreads();
-        long long before = sum;
-        for (int w = 0; w < warp; w++) before += s.sums[w + 1];
-        __syncthreads();
-        s.sums[threadIdx.x + 1] = before;
-        if (threadIdx.x == 0) s.sums[0] = 0;
-        __syncthreads();
-        records = s.sums[kThreads];
-    }
-    // the CTA's records and, of them, this warp's
-    const Shares of_ctas(records, gridDim.x);
-    const long long cta_begin = of_ctas.start(blockIdx.x), cta_end = of_ctas.start(blockIdx.x + 1);
-    const Shares of_warps(cta_end - cta_begin, kWarps);
-    const long long begin = cta_begin + of_warps.start(warp), end = cta_begin + of_warps.start(warp + 1);
-    long long item_at = 0;  // record index of the current item's first page
+    long long records = 0, cta_begin = 0, cta_end, begin, end;  // the call's records; of them the CTA's, and this warp's
+    long long item_at = 0;                                      // record index of the current item's first page
     int len = 0;
-    if (begin < end) {
+    if (a.whole) {  // a CTA an item, whose records count from 0
+        cur.row = blockIdx.x / virtual_heads, cur.item = blockIdx.x - cur.row * virtual_heads;
+        row_pages(a, cur.row, cur.first, cur.last);
+        cta_end = cur.last - cur.first;
+        const Shares of_warps(cta_end, kWarps);
+        begin = of_warps.start(warp), end = of_warps.start(warp + 1);
+        cur.page = cur.first + (int)begin;
+        len = a.row_len[cur.row];
+    } else {
+        // Records before each row.  Up to 32 rows: every warp scans them by itself, lane = row.  More: a thread sums a
+        // run of rows, the CTA scans the runs.
+        const auto row_records = [&](int row) {
+            int first, last;
+            row_pages(a, row, first, last);
+            return (long long)(last - first) * virtual_heads;
+        };
+        const auto scan = [&](long long x) {  // over the warp, this lane included
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const long long up = __shfl_up_sync(0xffffffffu, x, o);
+                if (lane >= o) x += up;
+            }
+            return x;
+        };
+        long long at = 0;  // records before the first one's row
+        long long upto = 0, mine = 0;
         if (a.rows <= 32) {
-            cur.row = __ffs(__ballot_sync(0xffffffffu, upto > begin)) - 1;
-            at = __shfl_sync(0xffffffffu, upto - mine, cur.row);
+            mine = lane < a.rows ? row_records(lane) : 0, upto = scan(mine);
+            records = __shfl_sync(0xffffffffu, upto, 31);
         } else {
             const int run = (a.rows + kThreads - 1) / kThreads;
-            int lo = 0, hi = kThreads;  // the run: sums[lo] <= begin < sums[hi]
-            while (hi - lo > 1) {
-                const int mid = (lo + hi) >> 1;
-                if (s.sums[mid] <= begin) lo = mid;
-                else hi = mid;
-            }
-            at = s.sums[lo];
-            for (cur.row = lo * run;; cur.row++) {
-                const long long n = row_records(cur.row);
-                if (begin < at + n) break;
-                at += n;
-            }
+            for (int i = threadIdx.x * run; i < min(a.rows, (int)(threadIdx.x + 1) * run); i++) mine += row_records(i);
+            const long long sum = scan(mine);
+            if (lane == 31) s.sums[warp + 1] = sum;
+            __syncthreads();
+            long long before = sum;
+            for (int w = 0; w < warp; w++) before += s.sums[w + 1];
+            __syncthreads();
+            s.sums[threadIdx.x + 1] = before;
+            if (threadIdx.x == 0) s.sums[0] = 0;
+            __syncthreads();
+            records = s.sums[kThreads];
         }
-        row_pages(a, cur.row, cur.first, cur.last);
-        const int pages = cur.last - cur.first;
-        cur.item = (int)quotient(begin - at, pages);
-        item_at = at + (long long)cur.item * pages;
-        cur.page = cur.first + (int)(begin - item_at);
-        len = a.row_len[cur.row];
+        const Shares of_ctas(records, gridDim.x);
+        cta_begin = of_ctas.start(blockIdx.x), cta_end = of_ctas.start(blockIdx.x + 1);
+        const Shares of_warps(cta_end - cta_begin, kWarps);
+        begin = cta_begin + of_warps.start(warp), end = cta_begin + of_warps.start(warp + 1);
+        if (begin < end) {
+            if (a.rows <= 32) {
+                cur.row = __ffs(__ballot_sync(0xffffffffu, upto > begin)) - 1;
+                at = __shfl_sync(0xffffffffu, upto - mine, cur.row);
+            } else {
+                const int run = (a.rows + kThreads - 1) / kThreads;
+                int lo = 0, hi = kThreads;  // the run: sums[lo] <= begin < sums[hi]
+                while (hi - lo > 1) {
+                    const int mid = (lo + hi) >> 1;
+                    if (s.sums[mid] <= begin) lo = mid;
+                    else hi = mid;
+                }
+                at = s.sums[lo];
+                for (cur.row = lo * run;; cur.row++) {
+                    const long long n = row_records(cur.row);
+                    if (begin < at + n) break;
+                    at += n;
+                }
+            }
+            row_pages(a, cur.row, cur.first, cur.last);
+            const int pages = cur.last - cur.first;
+            cur.item = (int)quotient(begin - at, pages);
+            item_at = at + (long long)cur.item * pages;
+            cur.page = cur.first + (int)(begin - item_at);
+            len = a.row_len[cur.row];
+        }
     }
+
+    if (threadIdx.x == 0) s.begin = cta_begin, s.end = cta_end, s.records = records;  // for the end
 
     // the copies' own place, ahead of the reading
     SplitCursor ahead = cur;
@@ -583,9 +603,9 @@ __global__ void __launch_bounds__(SplitShape<kWide, sizeof(T) == 4>::kThreads, 1
         for (int i = 0; i < kSplitStages; i++)
             if (!(bad >> i & 1)) mbar_wait_bounded(&s.full[warp][i], phases >> i & 1, kSplitWait);
     }
-    if (threadIdx.x == 0) {
+    if (!a.whole && threadIdx.x == 0) {
         a.over[blockIdx.x].row = -1;
-        if (blockIdx.x == 0) a.over[kSplitCtas].end = records;
+        if (blockIdx.x == 0) a.over[kSplitCtas].end = s.records;
     }
     __syncthreads();
 
@@ -596,7 +616,7 @@ __global__ void __launch_bounds__(SplitShape<kWide, sizeof(T) == 4>::kThreads, 1
         if (it.row < 0 || (slot == 0 && warp > 0 && it.begin < begin)) continue;
         int last = warp;
         while (last + 1 < kWarps && s.info[last + 1][0].row >= 0 && s.info[last + 1][0].begin == it.begin) last++;
-        const bool whole = it.begin >= cta_begin && it.end <= cta_end;
+        const bool whole = it.begin >= s.begin && it.end <= s.end;
         const int kv = it.item / a.blocks, block = it.item - kv * a.blocks;
         const int heads = min(kHeadBlock, a.group - block * kHeadBlock);
         for (int h = 0; h < heads; h++) {
@@ -610,12 +630,12 @@ __global__ void __launch_bounds__(SplitShape<kWide, sizeof(T) == 4>::kThreads, 1
                            ((size_t)kv * a.group + block * kHeadBlock + h) * kHeadDim + 2 * lane,
                        j.o0 / j.sum, j.o1 / j.sum);
             } else {
-                float *dst = a.pieces + (((size_t)blockIdx.x * 2 + (it.begin > cta_begin)) * a.piece_heads + h) * kPieceHead;
+                float *dst = a.pieces + (((size_t)blockIdx.x * 2 + (it.begin > s.begin)) * a.piece_heads + h) * kPieceHead;
                 *reinterpret_cast<float2 *>(dst + 2 * lane) = make_float2(j.o0 / j.sum, j.o1 / j.sum);
                 if (lane == 0) *reinterpret_cast<float2 *>(dst + kHeadDim) = make_float2(j.top, j.sum);
             }
         }
-        if (!whole && it.begin < cta_begin && lane == 0) a.over[blockIdx.x] = it;
+        if (!whole && it.begin < s.begin && lane == 0) a.over[blockIdx.x] = it;
     }
     // rows that read nothing
     for (int row = blockIdx.x * kWarps + warp; row < a.rows; row += gridDim.x * kWarps) {
@@ -722,8 +742,12 @@ extern "C" NDL_API int ndl_attention_split(const void *q, long long q_stride, in
     NDL_REQUIRE(aligned(workspace, 16) && workspace && workspace_bytes >= need, "workspace of %zu bytes, %zu needed",
                 workspace_bytes, need);
     const int group = heads / kv_heads;
+    const int blocks = (group + kHeadBlock - 1) / kHeadBlock;
+    const int pages = window && window / kPagePositions + 2 < max_pages ? window / kPagePositions + 2 : max_pages;
+    const long long items = (long long)rows * kv_heads * blocks;
+    const bool whole = pages <= kWholePages && items <= kSplitCtas;
     SplitArgs a{q, out, q_stride, out_stride, row_slot, row_len, rows, heads, group,
-                (group + kHeadBlock - 1) / kHeadBlock, window, group < kHeadBlock ? group : kHeadBlock, scale,
+                blocks, window, group < kHeadBlock ? group : kHeadBlock, whole, scale,
                 {page_table, const_cast<uint8_t *>(pool), (long long)page_bytes, slots, max_pages, num_pages, layer,
                  kv_heads, status},
                 static_cast<SplitItem *>(workspace),
@@ -748,9 +772,9 @@ extern "C" NDL_API int ndl_attention_split(const void *q, long long q_stride, in
         });
         if (st != NDL_OK) return st;
         const int threads = wide ? SplitShape<true, sizeof(T) == 4>::kThreads : SplitShape<false, sizeof(T) == 4>::kThreads;
-        kernel<<<kSplitCtas, threads, smem, (cudaStream_t)stream>>>(a);
+        kernel<<<whole ? (unsigned)items : kSplitCtas, threads, smem, (cudaStream_t)stream>>>(a);
         const int rc2 = check_launch("attention_split");
-        if (rc2 != NDL_OK) return rc2;
+        if (rc2 != NDL_OK || whole) return rc2;
         PdlScope early(true);  // the join's launch overlaps the kernel above; it waits for its end before reading
         launch_kernel(attention_join_kernel<T>, dim3(kSplitCtas - 1, a.piece_heads), dim3(kJoinThreads), 0,
                       (cudaStream_t)stream, a, kSplitCtas);

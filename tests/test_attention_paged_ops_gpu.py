@@ -51,6 +51,23 @@ def test_split_matches_64_bits(ops, cuda, kind, heads, kv_heads):
 
 
 @pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("rows,heads,kv_heads,window", [(1, 8, 8, 0), (24, 34, 2, 0), (33, 6, 3, 0), (148, 4, 1, 0),
+                                                        (149, 4, 1, 0), (1, 4, 2, 800), (36, 34, 2, 100), (49, 3, 3, 1)])
+def test_split_of_short_rows(ops, cuda, kind, rows, heads, kv_heads, window):
+    """Short slots, or a short window of long ones, as many items as SMs and one more: no row reads more than 16
+    pages."""
+    rng = np.random.default_rng(rows + heads)
+    lengths = [int(n) for n in rng.integers(0, 1500 if window else 1025, rows)]
+    cache = Cache(rows, lengths, kv_heads, spare_columns=0)
+    if not window:
+        assert cache.max_pages <= 16
+    q, x = _queries(cache, kind, rows, heads, cuda)
+    out = ops.attention_split(q, _i32(range(rows), cuda), _i32(lengths, cuda), kv_heads, *cache.device(cuda), window=window)
+    for r, n in enumerate(lengths):
+        _check(kind, out[r], cache, r, x[r], n - 1, window)
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
 @pytest.mark.parametrize("rows,length", [(1, 20000), (2, 9001), (3, 4097), (9, 2050)])
 def test_split_of_long_rows(ops, cuda, kind, rows, length):
     lengths = [length - 37 * r for r in range(rows)]
