@@ -13,10 +13,11 @@
 // one another inside a 16-position chunk of a page (a run) then move their keys
 // as 16-byte chunks and their values 4 positions of a dim at a time (4x4 bytes
 // by permutes); others, as a decode step has them, go by words and bytes.
-// 16384 rows of 8 heads, bf16, most in runs: 55 us written and read back (floor
-// 16; 109 when every row went by words and bytes): what is left are the runs'
-// ragged ends and the single rows, whose value bytes take a sector each.  64
-// rows, fp32: 8 us each way, a launch and three dependent trips to memory.
+// 16384 rows of 8 heads, bf16, all but 1243 in runs: 53 us written and read back
+// (floor 16; 109 when every row went by words and bytes).  A CTA waits for its
+// rows' places, then for the rows; the single rows' value bytes take a sector
+// each, read and written whole (40 MB, some 9 us at the end).  64 rows, fp32: 8
+// us each way, a launch and three dependent trips to memory.
 #include "paged.cuh"
 
 namespace ndl {
@@ -52,6 +53,12 @@ struct KvRowsArgs {
 };
 
 constexpr int kRowWarps = 2, kRowThreads = 32 * kRowWarps;
+// CTAs an SM: waits for memory fill a CTA's time, so as many as registers allow, short of spills (16384 rows of runs, bf16,
+// with 10, 12, 14 and 16: append 22.3, 21.5, 20.8 and 20.9 us, gather 16.2, 16.3, 15.0 and 14.8).
+template <class T>
+constexpr int kAppendCtas = sizeof(T) == 4 ? 10 : 12;
+template <class T>
+constexpr int kGatherCtas = sizeof(T) == 4 ? 10 : 16;
 constexpr int kBlockRows = 32;           // rows of a block, at most
 constexpr int kChunk = 16;               // positions of a chunk: 16 bytes of a value dim
 constexpr int kSeenRows = kBlockRows + kChunk;  // and of the runs that start in it: a run is the block's it starts in
@@ -233,7 +240,7 @@ __device__ __forceinline__ int kv_row(const KvRowsSmem &s, const KvTask &t, int 
 }
 
 template <class T>
-__global__ void __launch_bounds__(kRowThreads, 10) kv_append_kernel(KvRowsArgs a) {
+__global__ void __launch_bounds__(kRowThreads, kAppendCtas<T>) kv_append_kernel(KvRowsArgs a) {
     __shared__ KvRowsSmem s;
     const int first = blockIdx.x * a.block_rows, head = blockIdx.y;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -334,7 +341,7 @@ __global__ void __launch_bounds__(kRowThreads, 10) kv_append_kernel(KvRowsArgs a
 }
 
 template <class T>
-__global__ void __launch_bounds__(kRowThreads, 10) kv_gather_kernel(KvRowsArgs a) {
+__global__ void __launch_bounds__(kRowThreads, kGatherCtas<T>) kv_gather_kernel(KvRowsArgs a) {
     __shared__ KvRowsSmem s;
     const int first = blockIdx.x * a.block_rows, head = blockIdx.y;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
