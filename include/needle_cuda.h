@@ -249,9 +249,9 @@ NDL_API int ndl_kv_gather(const int32_t *row_slot, const int32_t *row_pos, int r
  *   out = sum_j softmax_j(scale * q . k_j) v_j
  * Scores, softmax and sums are in fp32.  The products' operands are fp16,
  * scaled by powers of two: for bf16 keys, values (code * scale) and
- * probabilities round to one each; for fp16 the keys have two parts and the
- * value scales go to the probabilities; for fp32 queries and probabilities
- * have two parts too.  out may be q.  Rows of no sequence are left as they
+ * probabilities round to one each; for fp16 codes are exact, key scales
+ * multiply scores and value scales the probabilities, which round; for fp32
+ * queries and probabilities have two parts too.  out may be q.  Rows of no sequence are left as they
  * are; a sequence whose offsets descend or leave [0, rows] is skipped with
  * status 2, and so may be those behind it. */
 NDL_API int ndl_attention_prompt(const void *q, long long q_stride, int type, const int32_t *seq_rows,
@@ -263,9 +263,8 @@ NDL_API int ndl_attention_prompt(const void *q, long long q_stride, int type, co
 /* Attention of single tokens: row r attends to positions [0, row_len[r]) of
  * slot row_slot[r] (the last `window` of them with window > 0), its cache
  * split over several thread blocks and the parts joined.  A row of length 0
- * gives zeros.  Arithmetic as ndl_attention_prompt, but for the operands:
- * codes are exact in them, the key scales multiply scores, the value scales
- * probabilities, for every type.  out may be q.  workspace: device
+ * gives zeros.  Arithmetic as ndl_attention_prompt, for bf16 as for fp16.
+ * out may be q.  workspace: device
  * memory of ndl_attention_split_workspace bytes, 16-byte aligned; calls that
  * overlap on the GPU need one each.  Its contents need no set-up and mean
  * nothing between calls. */

@@ -53,22 +53,9 @@ __device__ __forceinline__ uint32_t half_rest(float a, float b, uint32_t pair) {
     return half_pair(a - f.x, b - f.y);
 }
 
-// Four int8 codes of a word times a scale as two pairs of fp16, and what the
-// pairs' rounding left.  The code is exact in fp32: the biased byte in the low
-// mantissa bits of 2^23, less 2^23 + 128.
-__device__ __forceinline__ void scaled_codes(uint32_t w, float scale, uint32_t &a, uint32_t &b, uint32_t &ra,
-                                             uint32_t &rb) {
-    const uint32_t u = w ^ 0x80808080u;
-    const uint64_t bias = f2_pack(-8388736.0f, -8388736.0f), s2 = f2_pack(scale, scale);
-    const auto byte = [&](int sel) { return __uint_as_float(__byte_perm(u, 0x4B000000u, 0x7440 + sel)); };
-    float f0, f1, f2, f3;
-    f2_unpack(f2_mul(f2_add(f2_pack(byte(0), byte(1)), bias), s2), f0, f1);
-    f2_unpack(f2_mul(f2_add(f2_pack(byte(2), byte(3)), bias), s2), f2, f3);
-    a = half_pair(f0, f1), b = half_pair(f2, f3);
-    ra = half_rest(f0, f1, a), rb = half_rest(f2, f3, b);
-}
-// The same in one fp16 each, by a scale given as two fp16 (its rounding and
-// the rest, each twice): two roundings of the product.
+// Four int8 codes of a word times a scale as two pairs of fp16, the scale given
+// as two fp16 (its rounding and the rest, each twice): two roundings of the
+// product.
 __device__ __forceinline__ void folded_codes(uint32_t w, uint32_t scale, uint32_t rest, uint32_t &a, uint32_t &b) {
     codes_to_half(w, a, b);
     a = half2_bits(__hfma2(as_half2(a), as_half2(rest), __hmul2(as_half2(a), as_half2(scale))));

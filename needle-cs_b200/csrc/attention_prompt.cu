@@ -9,20 +9,22 @@
 //   S = Q K^T       tcgen05.mma, fp16 operands, fp32 accumulator in TMEM
 //   e = 2^(f S - m),  l += e,  P = e,  O += P V
 // Every operand is brought into fp16's range by a power of two: a query row's
-// largest element to [2^10, 2^11) (16-bit queries stay exact), the keys of a
-// step to below 2^15 (f undoes both), the values to below 2^15 by that of the
-// largest scale so far (O is rescaled where it grows).  m follows the true
-// maximum only where that is 7 binary orders above it, so O is rescaled on few
-// steps.  What an operand rounds to:
+// largest element to [2^10, 2^11) (16-bit queries stay exact), the key scales of
+// a step to below 2^8 (f undoes both), the value scales to below 2^8 by that of
+// the largest so far (O is rescaled where it grows).  m follows the true maximum
+// only where that is 7 binary orders above it, so O is rescaled on few steps.
+// What an operand rounds to:
 //   bf16  keys, values (code * scale) and P one fp16 each: 2^-11 a term, an
 //         eighth of the result's own rounding;
-//   fp16  keys in two parts (22 bits), values as bare codes (exact) with their
-//         scales on P, which rounds as the result does;
+//   fp16  keys and values as bare codes (exact), their scales on S and on P,
+//         which rounds as the result does;
 //   fp32  as fp16, and queries and P in two parts: 2^-21 throughout.
-// The key scales go into the operand because a scale a column costs the softmax
-// threads (thread = row) a shared-memory wavefront a column and warp: with both
-// scales there that pipe was as busy as the exponentials (8192 rows of 32 heads
-// over 8: 967 us then, 730 with the scales in the operands).
+// A scale a column costs the softmax threads (thread = row) a shared-memory
+// wavefront a column and warp, so for bf16 both go into the operands (8192 rows
+// of 32 heads over 8: 730 us against 967 with both on S and P, at the time).
+// Keys in two parts would keep one of the scales out of fp16's and fp32's
+// softmax at 4 and 8 more products a step: fp16 6 % faster over long prompts,
+// fp32 5 % slower.
 //
 // Warps: 4 softmax warps a tile (maximum and sum need no exchange), 4 that
 // convert pages (int8 records -> fp16 tiles in shared memory, 128-byte swizzled
@@ -36,8 +38,10 @@
 // the conversions.  The three tiles hide one another's waits: two took 524, two
 // with steps of 128 columns 545, one tile and two CTAs an SM 664.  Short prompts
 // are bound by what a CTA does around its steps (a step of three tiles takes 1.4
-// us, of fp32's two 1.6, all else 9 to 11) and by the CTAs that come last: 32
-// prompts of up to 384 rows, 8 heads, fp32: 40 us; one of 37 rows: 8 us.
+// to 1.7 us, of fp32's two 1.6, all else 9 to 11) and by the CTAs that come last:
+// 32 prompts of up to 384 rows, 8 heads, fp32: 40 us; one of 37 rows: 8 us.
+// (Two threads a row of fp32, each with half the columns and an output of its
+// own, took as long a step and 1 us more around them.)
 //
 // A value scale that is no number would reach rows that do not see its
 // position through the product (0 * NaN): it is replaced by 0 and its key
@@ -62,8 +66,8 @@ constexpr int kConvertWarps = 4;
 template <class T>
 struct Step {
     static constexpr bool kSplit = sizeof(T) == 4;                       // queries and P in two parts
-    static constexpr bool kFoldValues = __is_same(T, __nv_bfloat16);     // value scales on the values, else on P
-    static constexpr int kQParts = kSplit ? 2 : 1, kKParts = kFoldValues ? 1 : 2;
+    static constexpr bool kFold = __is_same(T, __nv_bfloat16);           // scales on keys and values, else on S and P
+    static constexpr int kQParts = kSplit ? 2 : 1;
     // Tiles of 128 rows: three (above); the softmax of fp32, with a second part of each probability, needs the
     // registers of two.
     static constexpr int kTiles = kSplit ? 2 : 3, kRows = kTiles * kTileRows;
@@ -102,10 +106,10 @@ template <class T>
 struct PromptSmem {
     using St = Step<T>;
     uint8_t q[St::kTiles][St::kQParts][kTileBytes];  // 1024-byte aligned
-    uint8_t k[St::kStages][St::kKParts][St::kPages][kPageTile], v[St::kStages][St::kPages][kPageTile];
+    uint8_t k[St::kStages][St::kPages][kPageTile], v[St::kStages][St::kPages][kPageTile];
     uint8_t raw[St::kRaw][St::kPages][kKvBlockBytes];
     float scales[kConvertWarps][2][St::kPages][kPagePositions];  // each converter warp's copy: keys, values
-    float vs[St::kStages][St::kFoldValues ? 4 : St::kCols];
+    __align__(16) float ks[St::kStages][St::kFold ? 4 : St::kCols], vs[St::kStages][St::kFold ? 4 : St::kCols];
     float key_factor[St::kStages];  // 2^(the keys' exponent), the scale of their scores
     int exponent[St::kStages];      // of the value scales so far
     uint64_t raw_full[St::kRaw], kv_full[St::kStages], kv_empty[St::kStages];
@@ -337,6 +341,18 @@ __global__ void __launch_bounds__(Step<T>::kThreads, 1) attention_prompt_kernel(
             if (lane == 0) mbar_arrive(&s.s_free[t]);
             // has the previous product read P and finished O?  (asked ahead: the answer takes some 70 clocks)
             const bool pv_ready = it == 0 || mbar_test_wait(&s.pv_done[t], (it - 1) & 1);
+            if constexpr (!St::kFold) {  // the key scales
+                const ulonglong2 *ks = reinterpret_cast<const ulonglong2 *>(s.ks[st]);
+#pragma unroll
+                for (int j = 0; j < kCols; j += 4) {
+                    const ulonglong2 k2 = ks[j / 4];
+                    float x[4];
+                    f2_unpack(f2_mul(f2_pack(__uint_as_float(r[j]), __uint_as_float(r[j + 1])), k2.x), x[0], x[1]);
+                    f2_unpack(f2_mul(f2_pack(__uint_as_float(r[j + 2]), __uint_as_float(r[j + 3])), k2.y), x[2], x[3]);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) r[j + e] = __float_as_uint(x[e]);
+                }
+            }
             if (!whole) {
 #pragma unroll
                 for (int j = 0; j < kCols; j++)
@@ -356,7 +372,7 @@ __global__ void __launch_bounds__(Step<T>::kThreads, 1) attention_prompt_kernel(
             if (ke > exponent) keep *= exp2_approx((float)(exponent - ke));
             exponent = ke;
             // folded value scales leave P room up to 2^15
-            const float base = (top == -INFINITY ? 0.0f : top) - (St::kFoldValues ? 8.0f : 0.0f);
+            const float base = (top == -INFINITY ? 0.0f : top) - (St::kFold ? 8.0f : 0.0f);
             [[maybe_unused]] const ulonglong2 *vs = reinterpret_cast<const ulonglong2 *>(s.vs[st]);
             const uint64_t f2 = f2_pack(f, f), base2 = f2_pack(-base, -base);
             uint64_t sums[2] = {0, 0};
@@ -365,7 +381,7 @@ __global__ void __launch_bounds__(Step<T>::kThreads, 1) attention_prompt_kernel(
 #pragma unroll
             for (int j = 0; j < kCols; j += 4) {
                 [[maybe_unused]] ulonglong2 v2;
-                if constexpr (!St::kFoldValues) v2 = vs[j / 4];
+                if constexpr (!St::kFold) v2 = vs[j / 4];
 #pragma unroll
                 for (int u = 0; u < 2; u++) {
                     const int k = j + 2 * u;
@@ -374,7 +390,7 @@ __global__ void __launch_bounds__(Step<T>::kThreads, 1) attention_prompt_kernel(
                     e0 = exp2_approx(e0), e1 = exp2_approx(e1);
                     const uint64_t e = f2_pack(e0, e1);
                     sums[u] = f2_add(sums[u], e);
-                    if constexpr (!St::kFoldValues) f2_unpack(f2_mul(e, u ? v2.y : v2.x), e0, e1);
+                    if constexpr (!St::kFold) f2_unpack(f2_mul(e, u ? v2.y : v2.x), e0, e1);
                     hp[k / 2] = half_pair(e0, e1);
                     if constexpr (kSplit) lp[kSplit ? k / 2 : 0] = half_rest(e0, e1, hp[k / 2]);
                 }
@@ -495,13 +511,12 @@ __global__ void __launch_bounds__(Step<T>::kThreads, 1) attention_prompt_kernel(
                 for (int h = 0; h < 2; h++) {
                     const int p = lane + 32 * h;
                     const float k = ks[g][h] * key_norm, v = vs[g][h] * value_norm;
-                    if constexpr (St::kFoldValues) {  // the key scale as two fp16, the value scale as one
+                    if constexpr (St::kFold) {  // the key scale as two fp16, the value scale as one
                         const uint32_t kh = half_pair(k, 0.0f);
                         reinterpret_cast<uint32_t *>(s.scales[c][0][g])[p] = half_pair(k, k - __low2float(as_half2(kh)));
                         reinterpret_cast<__half *>(s.scales[c][1][g])[p] = __float2half_rn(v);
                     } else {
-                        s.scales[c][0][g][p] = k;
-                        if (c == 0) s.vs[st][g * kPagePositions + p] = v;
+                        if (c == 0) s.ks[st][g * kPagePositions + p] = k, s.vs[st][g * kPagePositions + p] = v;
                     }
                 }
             __syncwarp();
@@ -523,27 +538,29 @@ __global__ void __launch_bounds__(Step<T>::kThreads, 1) attention_prompt_kernel(
                 const int row = c * 16 + (lane & 7);
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
-                    const float sc = s.scales[c][0][g][row + 8 * h];
-                    const uint32_t sh = __byte_perm(__float_as_uint(sc), 0, 0x1010), sl = __byte_perm(__float_as_uint(sc), 0, 0x3232);
+                    uint32_t sh = 0, sl = 0;
+                    if constexpr (St::kFold) {
+                        const uint32_t sc = reinterpret_cast<const uint32_t *>(s.scales[c][0][g])[row + 8 * h];
+                        sh = __byte_perm(sc, 0, 0x1010), sl = __byte_perm(sc, 0, 0x3232);
+                    }
 #pragma unroll
                     for (int u = 0; u < 2; u++) {
                         // words: (row, dims), (row + 8, dims), then dims + 16
                         const uint32_t w0 = h ? kw[g][u].y : kw[g][u].x, w1 = h ? kw[g][u].w : kw[g][u].z;
                         const int at = (row + 8 * h) * 128 + (((u * 4 + (lane >> 3)) ^ (row & 7)) << 4);
-                        uint32_t hi[4], lo[4];
-                        if constexpr (St::kFoldValues) {
-                            folded_codes(w0, sh, sl, hi[0], hi[1]);
-                            folded_codes(w1, sh, sl, hi[2], hi[3]);
+                        uint32_t x[4];
+                        if constexpr (St::kFold) {
+                            folded_codes(w0, sh, sl, x[0], x[1]);
+                            folded_codes(w1, sh, sl, x[2], x[3]);
                         } else {
-                            scaled_codes(w0, sc, hi[0], hi[1], lo[0], lo[1]);
-                            scaled_codes(w1, sc, hi[2], hi[3], lo[2], lo[3]);
-                            *reinterpret_cast<uint4 *>(&s.k[st][St::kKParts - 1][g][at]) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                            codes_to_half(w0, x[0], x[1]);
+                            codes_to_half(w1, x[2], x[3]);
                         }
-                        *reinterpret_cast<uint4 *>(&s.k[st][0][g][at]) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                        *reinterpret_cast<uint4 *>(&s.k[st][g][at]) = make_uint4(x[0], x[1], x[2], x[3]);
                     }
                 }
                 uint32_t f[8];
-                if constexpr (St::kFoldValues) {
+                if constexpr (St::kFold) {
                     const uint4 *sc = reinterpret_cast<const uint4 *>(s.scales[c][1][g]) + (lane >> 3) * 2;
                     const uint4 s0 = sc[0], s1 = sc[1];
                     f[0] = s0.x, f[1] = s0.y, f[2] = s0.z, f[3] = s0.w, f[4] = s1.x, f[5] = s1.y, f[6] = s1.z, f[7] = s1.w;
@@ -554,7 +571,7 @@ __global__ void __launch_bounds__(Step<T>::kThreads, 1) attention_prompt_kernel(
                     uint32_t h[8];
 #pragma unroll
                     for (int j = 0; j < 4; j++) codes_to_half(words[j], h[2 * j], h[2 * j + 1]);
-                    if constexpr (St::kFoldValues) {
+                    if constexpr (St::kFold) {
 #pragma unroll
                         for (int j = 0; j < 8; j++) h[j] = half2_bits(__hmul2(as_half2(h[j]), as_half2(f[j])));
                     }
@@ -620,13 +637,11 @@ __global__ void __launch_bounds__(Step<T>::kThreads, 1) attention_prompt_kernel(
                 if (!ok) return;
                 tc_fence_after();
 #pragma unroll
-                for (int qp = 0; qp < St::kQParts; qp++)
+                for (int qp = 0; qp < St::kQParts; qp++) {
+                    const uint64_t q = sw128_kmajor_desc(s.q[t][qp]), b = sw128_kmajor_desc(s.k[st]);
 #pragma unroll
-                    for (int kp = 0; kp < St::kKParts - (qp ? 1 : 0); kp++) {  // not the second parts of both
-                        const uint64_t q = sw128_kmajor_desc(s.q[t][qp]), b = sw128_kmajor_desc(s.k[st][kp]);
-#pragma unroll
-                        for (int k = 0; k < 4; k++) mma_f16_ss(ts, q + 2 * k, b + 2 * k, idesc_s, qp + kp + k > 0);
-                    }
+                    for (int k = 0; k < 4; k++) mma_f16_ss(ts, q + 2 * k, b + 2 * k, idesc_s, qp + k > 0);
+                }
                 // the products' end, and (by a plain arrive) the converters' scales of the step, which this warp has seen
                 mma_commit_elect(&s.s_full[t]);
                 if (lane == 0) mbar_arrive(&s.s_full[t]);
