@@ -637,10 +637,10 @@ __global__ void __launch_bounds__(Step<T>::kThreads, 1) attention_prompt_kernel(
                 if (!ok) return;
                 tc_fence_after();
 #pragma unroll
-                for (int qp = 0; qp < St::kQParts; qp++) {
-                    const uint64_t q = sw128_kmajor_desc(s.q[t][qp]), b = sw128_kmajor_desc(s.k[st]);
+                for (int i = 0; i < St::kQParts; i++) {  // the small part first: the accumulator truncates what is added
+                    const uint64_t q = sw128_kmajor_desc(s.q[t][St::kQParts - 1 - i]), b = sw128_kmajor_desc(s.k[st]);
 #pragma unroll
-                    for (int k = 0; k < 4; k++) mma_f16_ss(ts, q + 2 * k, b + 2 * k, idesc_s, qp + k > 0);
+                    for (int k = 0; k < 4; k++) mma_f16_ss(ts, q + 2 * k, b + 2 * k, idesc_s, i + k > 0);
                 }
                 // the products' end, and (by a plain arrive) the converters' scales of the step, which this warp has seen
                 mma_commit_elect(&s.s_full[t]);

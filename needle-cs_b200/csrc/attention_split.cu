@@ -233,23 +233,26 @@ __device__ __forceinline__ void attend_page(const uint8_t *rec, uint8_t *prob, i
         for (int b = 0; b < NB; b++)
 #pragma unroll
             for (int i = 0; i < 4; i++) s[b][T][i] = 0.0f;
+        uint32_t x[2][8];
 #pragma unroll
         for (int k = 0; k < 2; k++) {
             // words: (row g, dims), (row g + 8, dims), then dims + 16
             const uint4 w = *reinterpret_cast<const uint4 *>(rec + T * 1024 + k * 512 + lane * 16);
-            uint32_t x[8];
-            codes_to_half(w.x, x[0], x[1]);
-            codes_to_half(w.y, x[2], x[3]);
-            codes_to_half(w.z, x[4], x[5]);
-            codes_to_half(w.w, x[6], x[7]);
-#pragma unroll
-            for (int b = 0; b < NB; b++)
-#pragma unroll
-                for (int part = 0; part < kParts; part++) {
-                    mma_16816(s[b][T], x[0], x[2], x[1], x[3], q.b[part][b][2 * k][0], q.b[part][b][2 * k][1]);
-                    mma_16816(s[b][T], x[4], x[6], x[5], x[7], q.b[part][b][2 * k + 1][0], q.b[part][b][2 * k + 1][1]);
-                }
+            codes_to_half(w.x, x[k][0], x[k][1]);
+            codes_to_half(w.y, x[k][2], x[k][3]);
+            codes_to_half(w.z, x[k][4], x[k][5]);
+            codes_to_half(w.w, x[k][6], x[k][7]);
         }
+        // the small part first: the accumulator truncates what is added
+#pragma unroll
+        for (int part = kParts - 1; part >= 0; part--)
+#pragma unroll
+            for (int k = 0; k < 2; k++)
+#pragma unroll
+                for (int b = 0; b < NB; b++) {
+                    mma_16816(s[b][T], x[k][0], x[k][2], x[k][1], x[k][3], q.b[part][b][2 * k][0], q.b[part][b][2 * k][1]);
+                    mma_16816(s[b][T], x[k][4], x[k][6], x[k][5], x[k][7], q.b[part][b][2 * k + 1][0], q.b[part][b][2 * k + 1][1]);
+                }
     }
     // the positions' scales: keys (2 T + h) in a row, values over 2^exponent (of the largest so far) times 2^8
     const bool whole = from <= 0 && upto >= kPagePositions;
