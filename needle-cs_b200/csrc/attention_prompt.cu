@@ -38,8 +38,8 @@
 // the conversions.  The three tiles hide one another's waits: two took 524, two
 // with steps of 128 columns 545, one tile and two CTAs an SM 664.  Short prompts
 // are bound by what a CTA does around its steps (a step of three tiles takes 1.4
-// to 1.7 us, of fp32's two 1.6, all else 9 to 11) and by the CTAs that come last:
-// 32 prompts of up to 384 rows, 8 heads, fp32: 40 us; one of 37 rows: 8 us.
+// to 1.7 us, of fp32's two 1.8, all else 9 to 11) and by the CTAs that come last:
+// 32 prompts of up to 384 rows, 8 heads, fp32: 41 us; one of 37 rows: 8 us.
 // (Two threads a row of fp32, each with half the columns and an output of its
 // own, took as long a step and 1 us more around them.)
 //
@@ -78,7 +78,11 @@ struct Step {
     // TMEM columns: scores, outputs, probabilities (two fp16 a column; fp32: then their second parts) of the tiles
     static constexpr int kS = 0, kO = kTiles * kCols, kP = kO + kTiles * kHeadDim, kPCols = kCols / 2;
     static constexpr int kLo = kTiles * kPCols;
-    static_assert(kP + kTiles * kPCols * (kSplit ? 2 : 1) <= kTmemCols, "TMEM columns");
+    // fp32: the accumulators truncate what is added, a bias that grows with the steps; so every kFlush steps O goes over
+    // to a sum, which rounds (a prompt of 1408 rows is off by 1.4e-6 without, 0.9e-6 with 8 steps, 0.6e-6 with 4; a
+    // time costs 1 us: a step takes 1.6 us without, 1.8 with 8 steps).
+    static constexpr int kFlush = kSplit ? 8 : 1, kSum = kLo + kP + kTiles * kPCols;
+    static_assert((kSplit ? kSum + kTiles * kHeadDim : kP + kTiles * kPCols) <= kTmemCols, "TMEM columns");
     // Warps: softmax, converters, then a group of one MMA warp a tile and one that copies.
     static constexpr int kConvertWarp = 4 * kTiles, kMmaWarp = kConvertWarp + kConvertWarps, kCopyWarp = kMmaWarp + 3;
     static constexpr int kThreads = 32 * (kMmaWarp + 4);
@@ -318,10 +322,12 @@ __global__ void __launch_bounds__(Step<T>::kThreads, 1) attention_prompt_kernel(
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t ts = tmem + lanes + St::kS + t * kCols, to = tmem + lanes + St::kO + t * kHeadDim;
         const uint32_t tp = tmem + lanes + St::kP + t * St::kPCols;
+        [[maybe_unused]] const uint32_t sum_at = tmem + lanes + St::kSum + t * kHeadDim;
         float top = -INFINITY, total = 0.0f;
+        [[maybe_unused]] float owed = 1.0f;  // what O was scaled by since the last time it went over to the sum
         int exponent = kMinExponent;
         bool ok = true;
-        for (int i = lo_t; i <= hi_t; i++) {
+        for (int i = lo_t; ok && i <= hi_t; i++) {
             const int it = i - lo_t, st = i % kStages;
             // positions [from, upto] of the step are this row's
             const int upto = max(pos - (page0 + i * kPages) * kPagePositions, -1);
@@ -413,6 +419,7 @@ __global__ void __launch_bounds__(Step<T>::kThreads, 1) attention_prompt_kernel(
                     for (int j = 0; j < 16; j++) o[j] = __float_as_uint(__uint_as_float(o[j]) * keep);
                     tmem_st16(to + c, o);
                 }
+                if constexpr (kSplit) owed *= keep;
             }
 #pragma unroll
             for (int c = 0; c < kCols / 2; c += 16) {
@@ -423,6 +430,27 @@ __global__ void __launch_bounds__(Step<T>::kThreads, 1) attention_prompt_kernel(
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&s.p_full[t]);
+            if constexpr (kSplit) {
+                if ((it + 1) % St::kFlush == 0 && i < hi_t) {  // O goes over to the sum
+                    ok = warp_wait(&s.pv_done[t], it & 1, &s.abort);
+                    tc_fence_after();
+#pragma unroll
+                    for (int c = 0; c < kHeadDim; c += 16) {
+                        uint32_t o[16], u[16];
+                        tmem_ld16(to + c, o);
+                        tmem_ld16(sum_at + c, u);  // (nothing yet at the first)
+                        tmem_ld_wait(o);
+                        tmem_ld_wait(u);
+#pragma unroll
+                        for (int j = 0; j < 16; j++)
+                            o[j] = __float_as_uint(__uint_as_float(o[j]) + (it >= St::kFlush ? __uint_as_float(u[j]) * owed : 0.0f));
+                        tmem_st16(sum_at + c, o);
+                    }
+                    tmem_st_wait();
+                    tc_fence_before();
+                    owed = 1.0f;
+                }
+            }
         }
         // the rows' results
         if (hi_t >= lo_t) {
@@ -437,6 +465,19 @@ __global__ void __launch_bounds__(Step<T>::kThreads, 1) attention_prompt_kernel(
             tmem_ld32(to + 32, r1);
             tmem_ld_wait(r0);
             tmem_ld_wait(r1);
+            if (kSplit && hi_t - lo_t >= St::kFlush) {
+#pragma unroll
+                for (int c = 0; c < kHeadDim; c += 16) {
+                    uint32_t u[16];
+                    tmem_ld16(sum_at + c, u);
+                    tmem_ld_wait(u);
+#pragma unroll
+                    for (int j = 0; j < 16; j++) {
+                        uint32_t &o = c < 32 ? r0[c + j] : r1[(c + j) & 31];
+                        o = __float_as_uint(__uint_as_float(o) + __uint_as_float(u[j]) * owed);
+                    }
+                }
+            }
             const float inverse = ok ? 1.0f / total : __int_as_float(0x7fc00000), back = pow2(exponent - 8);
             float x[64];
 #pragma unroll
@@ -656,11 +697,12 @@ __global__ void __launch_bounds__(Step<T>::kThreads, 1) attention_prompt_kernel(
                     if (!ok) break;
                     tc_fence_after();
 #pragma unroll
-                    for (int part = 0; part < (kSplit ? 2 : 1); part++)
+                    for (int i = 0; i < (kSplit ? 2 : 1); i++)  // the small part first
 #pragma unroll
                         for (int k = 0; k < 4 * kPages; k++)
-                            mma_f16_ts(to, tp + part * St::kLo + k * 8, sw128_kmajor_desc(s.v[st][k >> 2]) + 2 * (k & 3), idesc_o,
-                                       it + part + k > 0);
+                            mma_f16_ts(to, tp + (kSplit && i == 0 ? St::kLo : 0) + k * 8,
+                                       sw128_kmajor_desc(s.v[st][k >> 2]) + 2 * (k & 3), idesc_o,
+                                       (kSplit ? it % St::kFlush : it) + i + k > 0);
                     mma_commit_elect(&s.pv_done[t]);
                 } else {  // the step is other tiles' alone
                     ok = warp_wait(&s.kv_full[st], (i / kStages) & 1, &s.abort);

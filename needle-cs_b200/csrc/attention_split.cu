@@ -337,7 +337,13 @@ __device__ __forceinline__ void attend_page(const uint8_t *rec, uint8_t *prob, i
             for (int T = 0; T < 4; T++)
                 p[part][b][T] = *reinterpret_cast<const uint2 *>(prob + ((part * NB + b) * 8 + g) * kProbRow + (16 * T + 4 * t) * 2);
 #pragma unroll
-    for (int D = 0; D < 4; D++)
+    for (int D = 0; D < 4; D++) {
+        // (fp32: the parts of a page by themselves, then into the output by additions that round)
+        float part_o[kParts][NB][4];
+        if constexpr (kSplit) {
+#pragma unroll
+            for (int i = 0; i < kParts * NB * 4; i++) (&part_o[0][0][0])[i] = 0.0f;
+        }
 #pragma unroll
         for (int T = 0; T < 4; T += 2) {
             // matrices: dims 16 D + 0..7 and + 8..15 of chunk T, then of chunk T + 1
@@ -353,9 +359,17 @@ __device__ __forceinline__ void attend_page(const uint8_t *rec, uint8_t *prob, i
                 for (int b = 0; b < NB; b++)
 #pragma unroll
                     for (int part = 0; part < kParts; part++)
-                        mma_16816(st.o[b][D], x[0], x[2], x[1], x[3], p[part][b][T + u].x, p[part][b][T + u].y);
+                        mma_16816(kSplit ? part_o[part][b] : st.o[b][D], x[0], x[2], x[1], x[3], p[part][b][T + u].x,
+                                  p[part][b][T + u].y);
             }
         }
+        if constexpr (kSplit) {
+#pragma unroll
+            for (int b = 0; b < NB; b++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) st.o[b][D][i] += part_o[kParts - 1][b][i] + part_o[0][b][i];
+        }
+    }
     __syncwarp();  // the probabilities' place is free again
 }
 
