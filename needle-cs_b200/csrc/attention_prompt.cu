@@ -708,7 +708,7 @@ __global__ void __launch_bounds__(Step<T>::kThreads, 1) attention_prompt_kernel(
                     ok = warp_wait(&s.kv_full[st], (i / kStages) & 1, &s.abort);
                     if (!ok) break;
                 }
-                mma_commit_elect(&s.kv_empty[st]);
+                if (i + kStages < steps) mma_commit_elect(&s.kv_empty[st]);  // (no arrival that nobody waits for)
             }
             if (!ok) {  // every product in flight ends before the CTA's TMEM is freed (bounded)
                 mma_commit_elect(&s.drained[t]);
