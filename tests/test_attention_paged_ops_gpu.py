@@ -310,6 +310,39 @@ def test_prompt_of_long_sequences(ops, cuda, kind):
                 _check(kind, out[ends[s] + r], cache, s, x[ends[s] + r], prefixes[s] + r, window)
 
 
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("window", [0, 900])
+def test_prompt_whose_scores_and_scales_rise(ops, cuda, kind, window):
+    """The running maximum and the common power of two of the values move all along the row."""
+    cache = Cache(47, [1500], 2, layers=1, layer=0)
+    cache.ks[0] = (cache.ks[0] * np.linspace(1, 10, 1500)[:, None]).astype(np.float32)
+    cache.vs[0] = (cache.vs[0] * 2.0 ** (np.arange(1500) // 90)[:, None]).astype(np.float32)
+    _repack(cache)
+    q, x = _queries(cache, kind, 1000, 4, cuda)
+    out = ops.attention_prompt(q, _i32([0, 1000], cuda), _i32([0], cuda), _i32([500], cuda), 2, *cache.device(cuda),
+                               window=window)
+    for r in list(range(0, 1000, 61)) + [999]:
+        _check(kind, out[r], cache, 0, x[r], 500 + r, window)
+
+
+def test_long_fp32_sums_do_not_drift(ops, cuda):
+    """Equal weights and equal values: the result is the value.  Of the products' additions between two that round, at
+    most 64 (a prompt's 8 pages of 4 products in 2 parts), each loses less than 2^-23 of what the sum then is, i/64 of
+    it at the i-th: below 32 * 2^-23.  The 129 page sums and the total add up by roundings of 2^-24 of what they then
+    are, 65 * 2^-24 each at most, and weights, values and the quotient round within 2^-20.  Together below 2^-16."""
+    length = 8192 + 37
+    cache = Cache(48, [length], 1, layers=1, layer=0)
+    cache.v[0][:] = 127
+    cache.vs[0][:] = np.float32(0.0123)
+    _repack(cache)
+    want = 127.0 * float(np.float32(0.0123))
+    q = torch.zeros((40, 2, 64), device=cuda)
+    out = ops.attention_prompt(q, _i32([0, 40], cuda), _i32([0], cuda), _i32([length - 40], cuda), 1, *cache.device(cuda))
+    assert (out.double() / want - 1).abs().max().item() < 2.0 ** -16
+    out = ops.attention_split(q[:1], _i32([0], cuda), _i32([length], cuda), 1, *cache.device(cuda))
+    assert (out.double() / want - 1).abs().max().item() < 2.0 ** -16
+
+
 def test_prompt_rows_agree_with_single_tokens(ops, cuda):
     """Both operators within the bound of the same rows, over every row of a chunk."""
     cache = Cache(43, [170], 2)
